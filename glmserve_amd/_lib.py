@@ -37,6 +37,17 @@ SIGNATURES = {
     "glmmoe_fp8_layer_workspace_view": (_i, [_vp, _i, _vp, _vp]),
     "glmmoe_moe_layer_fp8": (_i, [_vp, _vp, _i, _vp, _vp, _sz, _vp]),
     "glmmoe_expert_ffn_fp8": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "glmmoe_grouped_linear": (_i, [_i, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i, _i64, _i64, _i64,
+                                   _i, _vp, _i64, _vp]),
+    "glmmoe_grouped_gate_up": (_i, [_i, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i, _i64, _i64,
+                                    _i64, _i, _vp, _i64, _vp]),
+    "glmmoe_lora_workspace_bytes": (_sz, [_i, _i, _i64, _i]),
+    "glmmoe_lora_add": (_i, [_i, _vp, _i64, _vp, _i, _i, _vp, _vp, _vp, _vp, _i, _i, _i64, _i64, _i,
+                             _vp, _i64, _vp, _i64, _vp, _sz, _vp]),
+    "glmmoe_bf16_layer_workspace_bytes": (_sz, [_vp, _i]),
+    "glmmoe_bf16_layer_workspace_view": (_i, [_vp, _i, _vp, _vp]),
+    "glmmoe_moe_layer_bf16": (_i, [_vp, _vp, _i, _vp, _vp, _sz, _vp]),
+    "glmmoe_expert_ffn_bf16": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
     "glmmoe_profile_enable": (_i, [_i]),
     "glmmoe_profile_read": (_i, [_vp, _vp]),
     "glmmoe_ref_register_w4a16": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
@@ -102,6 +113,22 @@ class Fp8Ws(C.Structure):
                 ("topk_w", _vp), ("expert_offsets", _vp), ("sorted_token_ids", _vp),
                 ("sorted_row", _vp), ("inv", _vp), ("tiles", _vp), ("ntiles", _vp),
                 ("hq", _vp), ("hscale", _vp), ("dpart", _vp), ("bytes", _sz)]
+
+
+class Bf16Layer(C.Structure):
+    """glmmoe_bf16_layer (include/glmmoe.h)."""
+    _fields_ = [("hidden", _i), ("moe_inter", _i), ("n_experts", _i), ("topk", _i),
+                ("norm_topk", _i), ("routed_scale", _f), ("router_w", _vp), ("e_bias", _vp),
+                ("gate", _vp), ("up", _vp), ("down", _vp), ("sh_gate", _vp), ("sh_up", _vp),
+                ("sh_down", _vp)]
+
+
+class Bf16Ws(C.Structure):
+    """glmmoe_bf16_ws (include/glmmoe.h)."""
+    _fields_ = [("logits", _vp), ("rpart", _vp), ("topk_ids", _vp), ("topk_w", _vp),
+                ("expert_offsets", _vp), ("sorted_token_ids", _vp), ("sorted_row", _vp),
+                ("inv", _vp), ("tiles", _vp), ("ntiles", _vp), ("h", _vp), ("dpart", _vp),
+                ("bytes", _sz)]
 
 
 _LIB = None

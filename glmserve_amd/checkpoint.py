@@ -1,5 +1,5 @@
-"""Checkpoint ingestion: one MoE layer of a glmserve W4 safetensors checkpoint
-onto the device as a W4A16MoELayer.
+"""Checkpoint ingestion: one MoE layer of a glmserve safetensors checkpoint onto
+the device, as a W4A16MoELayer or, with experts="bf16", as a BF16MoELayer.
 
 The W4 format is the one `tools/convert_hf_to_glmserve.py:216-252` writes and
 `src/model_glm52.cpp:157-196` reads:
@@ -19,7 +19,8 @@ routed_scaling_factor, `src/config.cpp:60-68`) or keyword arguments.
 
 Files are read with safetensors' own loader (no pickled objects are ever
 loaded). Expert weights stored as plain float tensors are quantized with
-`quantize_w4`, the converter's rule.
+`quantize_w4`, the converter's rule, or kept in bf16 (experts="bf16": values of
+other float types are rounded to it; int4 linears are refused there).
 """
 import json
 import os
@@ -27,7 +28,7 @@ import os
 import torch
 
 from ._lib import GlmMoeError
-from .ops import W4A16MoELayer, pack_w4a16
+from .ops import BF16MoELayer, W4A16MoELayer, pack_w4a16
 
 GROUP = 128   # the int4 group size the kernels take
 
@@ -112,10 +113,24 @@ def _linear_w4(st, base, rows, K):
     return quantize_w4(w)
 
 
-def read_layer(path, layer, hidden=None, moe_inter=None, n_experts=None):
+def _linear_bf16(st, base, rows, K):
+    """bf16 [rows, K] of one float linear."""
+    if not st.has(base + ".weight"):
+        raise GlmMoeError(f"{base}: no float .weight (an int4 linear loads with experts=\"w4\")")
+    w = st.get(base + ".weight")
+    if tuple(w.shape) != (rows, K) or not w.is_floating_point() or w.element_size() < 2:
+        raise GlmMoeError(f"{base}.weight: expected bf16, fp16 or fp32 [{rows}, {K}], got {w.dtype} "
+                          f"{list(w.shape)}")
+    return w.to(torch.bfloat16)
+
+
+def read_layer(path, layer, hidden=None, moe_inter=None, n_experts=None, experts="w4"):
     """Host tensors of MoE layer `layer`: dict with router_w [E, H] fp32, e_bias [E]
     fp32 or None, gate/up/down = (q [E, rows, K/2] u8, s [E, rows, K/g] fp32), shared =
-    the same triple for the shared expert (E = 1) or None, and config."""
+    the same triple for the shared expert (E = 1) or None, and config. experts="bf16":
+    gate/up/down and the shared triple are bf16 [E, rows, K] tensors."""
+    if experts not in ("w4", "bf16"):
+        raise GlmMoeError(f"experts: expected \"w4\" or \"bf16\", got {experts!r}")
     st = _Store(path) if not isinstance(path, _Store) else path
     p = f"model.layers.{layer}."
     rname = p + "mlp.gate" if (st.has(p + "mlp.gate.weight") or st.has(p + "mlp.gate.qweight")) \
@@ -140,6 +155,8 @@ def read_layer(path, layer, hidden=None, moe_inter=None, n_experts=None):
                       else st.get(g0 + ".weight").shape[0])
 
     def stack(prefixes, rows, K):
+        if experts == "bf16":
+            return torch.stack([_linear_bf16(st, pre, rows, K) for pre in prefixes]).contiguous()
         qs, ss = zip(*[_linear_w4(st, pre, rows, K) for pre in prefixes])
         return torch.stack(qs).contiguous(), torch.stack(ss).contiguous()
 
@@ -157,18 +174,26 @@ def read_layer(path, layer, hidden=None, moe_inter=None, n_experts=None):
                 hidden=H, moe_inter=I, n_experts=E, config=st.config)
 
 
-def load_layer(path, layer, topk=None, norm_topk=None, routed_scale=None, device="cuda"):
+def load_layer(path, layer, topk=None, norm_topk=None, routed_scale=None, device="cuda",
+               experts="w4"):
     """W4A16MoELayer for MoE layer `layer` of a checkpoint: one .safetensors file,
     or a directory of shards with config.json. Routing constants default to
     config.json, else to top-8 / normalized / 2.5. The router weights are used in
-    bf16 (the layer's router GEMM is bf16 x bf16 in a fixed fp32 order)."""
-    t = read_layer(path, layer)
+    bf16 (the layer's router GEMM is bf16 x bf16 in a fixed fp32 order).
+    experts="bf16": a BF16MoELayer on the checkpoint's float expert weights."""
+    t = read_layer(path, layer, experts=experts)
     cfg = t["config"]
     topk = topk if topk is not None else int(cfg.get("num_experts_per_tok", 8))
     norm_topk = norm_topk if norm_topk is not None else bool(cfg.get("norm_topk_prob", True))
     routed_scale = routed_scale if routed_scale is not None else float(
         cfg.get("routed_scaling_factor", 2.5))
     H, I, E = t["hidden"], t["moe_inter"], t["n_experts"]
+    router_w = t["router_w"].to(torch.bfloat16).to(device).contiguous()
+    e_bias = t["e_bias"].to(device).contiguous() if t["e_bias"] is not None else None
+    if experts == "bf16":
+        sh = None if t["shared"] is None else tuple(m[0].to(device) for m in t["shared"])
+        return BF16MoELayer(H, I, E, topk, router_w, e_bias, t["gate"].to(device), t["up"].to(device),
+                            t["down"].to(device), sh, norm_topk=norm_topk, routed_scale=routed_scale)
     if t["shared"] is not None and t["shared"][0][0].shape[1] != I:
         raise GlmMoeError("shared expert intermediate size must equal moe_intermediate_size")
 
@@ -183,7 +208,5 @@ def load_layer(path, layer, topk=None, norm_topk=None, routed_scale=None, device
     if t["shared"] is not None:
         shared = (dev_pack(t["shared"][0], I, H), dev_pack(t["shared"][1], I, H),
                   dev_pack(t["shared"][2], H, I))
-    router_w = t["router_w"].to(torch.bfloat16).to(device).contiguous()
-    e_bias = t["e_bias"].to(device).contiguous() if t["e_bias"] is not None else None
     return W4A16MoELayer(H, I, E, topk, router_w, e_bias, gate, up, down, shared,
                          norm_topk=norm_topk, routed_scale=routed_scale)

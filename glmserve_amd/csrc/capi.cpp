@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include "../../include/glmmoe.h"
+#include "grouped.hpp"
 #include "kernels.hpp"
 
 using namespace glmmoe;
@@ -149,6 +150,59 @@ size_t carve8(const glmmoe_fp8_layer* L, int n, char* base, glmmoe_fp8_ws* v) {
     return off;
 }
 
+// bf16 experts: shape and pointer checks, workspace.
+int check_layer16(const glmmoe_bf16_layer* L, int n) {
+    if (!L || n < 0) return GLMMOE_ERR_ARG;
+    if (L->hidden <= 0 || L->moe_inter <= 0 || L->n_experts <= 0 || L->topk <= 0)
+        return GLMMOE_ERR_ARG;
+    if (L->hidden % 256 || L->moe_inter % 8 || L->hidden > 8192 || L->moe_inter > (1 << 20))
+        return GLMMOE_ERR_SHAPE;
+    if (L->n_experts > 512 || L->topk > 8 || L->topk > L->n_experts) return GLMMOE_ERR_SHAPE;
+    if (n > (1 << 24) / L->topk) return GLMMOE_ERR_SHAPE;   // the dispatch's limit
+    if (!L->gate || !L->up || !L->down) return GLMMOE_ERR_ARG;
+    const int sh = (L->sh_gate != nullptr) + (L->sh_up != nullptr) + (L->sh_down != nullptr);
+    if (sh != 0 && sh != 3) return GLMMOE_ERR_ARG;
+    for (const uint16_t* p : {L->gate, L->up, L->down, L->sh_gate, L->sh_up, L->sh_down})
+        if (reinterpret_cast<uintptr_t>(p) % 16) return GLMMOE_ERR_ARG;
+    return GLMMOE_OK;
+}
+
+inline bool has_shared(const glmmoe_bf16_layer* L) { return L->sh_gate != nullptr; }
+
+// Rows of a tile of the layer's grouped products.
+int tile_rows16(const glmmoe_bf16_layer* L, int n) {
+    return grouped_tile_rows((long)n * L->topk, L->n_experts);
+}
+
+size_t carve16(const glmmoe_bf16_layer* L, int n, char* base, glmmoe_bf16_ws* v) {
+    const int H = L->hidden, I = L->moe_inter, E = L->n_experts, k = L->topk;
+    const size_t nk = (size_t)n * k;
+    const size_t R = nk + (has_shared(L) ? (size_t)n : 0);
+    const size_t mt = n ? (size_t)max_tiles_for(n, k, E, has_shared(L), tile_rows16(L, n)) : 0;
+    size_t off = 0;
+    auto take = [&](size_t bytes) -> char* {
+        char* p = base ? base + off : nullptr;
+        off += align256(bytes);
+        return p;
+    };
+    glmmoe_bf16_ws w{};
+    w.logits = reinterpret_cast<float*>(take((size_t)n * E * 4));
+    w.rpart = reinterpret_cast<float*>(take(router_select_scratch_bytes(n, H, E)));
+    w.topk_ids = reinterpret_cast<int*>(take(nk * 4));
+    w.topk_w = reinterpret_cast<float*>(take(nk * 4));
+    w.expert_offsets = reinterpret_cast<int*>(take((size_t)(E + 2) * 4));
+    w.sorted_token_ids = reinterpret_cast<int*>(take(R * 4));
+    w.sorted_row = reinterpret_cast<int*>(take(R * 4));
+    w.inv = reinterpret_cast<int*>(take(nk * 4));
+    w.tiles = reinterpret_cast<int*>(take(mt * 16));
+    w.ntiles = reinterpret_cast<int*>(take(16));
+    w.h = reinterpret_cast<uint16_t*>(take(R * I * 2));
+    w.dpart = reinterpret_cast<float*>(take(R * H * 4));
+    w.bytes = off;
+    if (v) *v = w;
+    return off;
+}
+
 // ---- stage timing ring ------------------------------------------------------
 struct Prof {
     bool on = false;
@@ -245,6 +299,48 @@ int run_experts8(const glmmoe_fp8_layer* L, const uint16_t* x, int n, const int*
     if (rc) return rc;
     mark(GLMMOE_STAGE_COMBINE, s);
     rc = launch_combine(v.dpart, v.inv, w, n, k, H, sh, out, s, true);
+    if (rc) return rc;
+    end_call(s);
+    return GLMMOE_OK;
+}
+
+// bf16: dispatch, the two grouped products on the dispatch's tiles, the combine.
+int run_experts16(const glmmoe_bf16_layer* L, const uint16_t* x, int n, const int* ids,
+                  const float* w, float* out, const glmmoe_bf16_ws& v, hipStream_t s,
+                  bool dispatched = false) {
+    const int H = L->hidden, I = L->moe_inter, E = L->n_experts, k = L->topk;
+    const int sh = has_shared(L) ? 1 : 0;
+    const int T = tile_rows16(L, n);
+    mark(GLMMOE_STAGE_DISPATCH, s);
+    int rc = dispatched ? 0
+                        : launch_dispatch(ids, n, k, E, v.expert_offsets, v.sorted_token_ids,
+                                          v.sorted_row, v.inv, v.tiles, v.ntiles, T, sh, 1, s,
+                                          dispatch_scratch(v.rpart, L, n), 0);
+    if (rc) return rc;
+    GroupedArgs a{};
+    a.tiles = v.tiles, a.ntiles = v.ntiles;
+    a.max_tiles = max_tiles_for(n, k, E, sh, T);
+    a.tb = T / 16;
+    a.E = E;
+    a.rows = n * (k + sh);
+    a.x = x, a.ldx = H, a.x_rows = n, a.row_ids = v.sorted_token_ids;
+    a.w0 = L->gate, a.w1 = L->up, a.w_stride = (long)I * H;
+    a.s0 = L->sh_gate, a.s1 = L->sh_up;
+    a.N = I, a.K = H;
+    a.y = v.h, a.ldy = I;
+    mark(GLMMOE_STAGE_GATE_UP, s);
+    rc = launch_grouped(a, GLMMOE_BF16, false, s);
+    if (rc) return rc;
+    a.x = v.h, a.ldx = I, a.x_rows = a.rows, a.row_ids = nullptr;
+    a.w0 = L->down, a.w1 = nullptr;
+    a.s0 = L->sh_down, a.s1 = nullptr;
+    a.N = H, a.K = I;
+    a.y = v.dpart, a.ldy = H;
+    mark(GLMMOE_STAGE_DOWN, s);
+    rc = launch_grouped(a, GLMMOE_BF16, true, s);
+    if (rc) return rc;
+    mark(GLMMOE_STAGE_COMBINE, s);
+    rc = launch_grouped_combine(v.dpart, v.inv, ids, w, n, k, E, H, sh, out, s);
     if (rc) return rc;
     end_call(s);
     return GLMMOE_OK;
@@ -532,6 +628,62 @@ int glmmoe_expert_ffn_fp8(const glmmoe_fp8_layer* L, const uint16_t* x, int n,
     begin_call();
     mark(GLMMOE_STAGE_ROUTER_LOGITS, S(stream));   // the activation quantization
     return run_experts8(L, x, n, topk_ids, topk_w, out, v, S(stream));
+}
+
+size_t glmmoe_bf16_layer_workspace_bytes(const glmmoe_bf16_layer* L, int n) {
+    if (check_layer16(L, n)) return 0;
+    return carve16(L, n, nullptr, nullptr);
+}
+
+int glmmoe_bf16_layer_workspace_view(const glmmoe_bf16_layer* L, int n, void* workspace,
+                                     glmmoe_bf16_ws* view) {
+    const int rc = check_layer16(L, n);
+    if (rc) return rc;
+    if (!workspace || !view) return GLMMOE_ERR_ARG;
+    carve16(L, n, static_cast<char*>(workspace), view);
+    return GLMMOE_OK;
+}
+
+int glmmoe_moe_layer_bf16(const glmmoe_bf16_layer* L, const uint16_t* x, int n, float* out,
+                          void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_layer16(L, n);
+    if (rc) return rc;
+    if (n == 0) return GLMMOE_OK;   // no tokens: nothing to compute or write
+    if (!x || !out || !workspace || !L->router_w) return GLMMOE_ERR_ARG;
+    if (reinterpret_cast<uintptr_t>(x) % 16 || reinterpret_cast<uintptr_t>(workspace) % 16)
+        return GLMMOE_ERR_ARG;
+    glmmoe_bf16_ws v;
+    if (carve16(L, n, static_cast<char*>(workspace), &v) > workspace_bytes)
+        return GLMMOE_ERR_WORKSPACE;
+    hipStream_t s = S(stream);
+    begin_call();
+    mark(GLMMOE_STAGE_ROUTER_LOGITS, s);
+    const DispOut disp{v.expert_offsets, v.sorted_token_ids, v.sorted_row, v.inv,
+                       reinterpret_cast<int4*>(v.tiles), v.ntiles, tile_rows16(L, n),
+                       has_shared(L) ? 1 : 0, 1, 0, nullptr, 0};
+    bool dispatched = false;
+    rc = launch_router_select(x, L->router_w, L->e_bias, n, L->hidden, L->n_experts, L->topk,
+                              L->norm_topk, L->routed_scale, v.logits, nullptr, v.rpart,
+                              v.topk_ids, v.topk_w, s, &disp, &dispatched);
+    if (rc) return rc;
+    mark(GLMMOE_STAGE_ROUTER_TOPK, s);
+    return run_experts16(L, x, n, v.topk_ids, v.topk_w, out, v, s, dispatched);
+}
+
+int glmmoe_expert_ffn_bf16(const glmmoe_bf16_layer* L, const uint16_t* x, int n,
+                           const int* topk_ids, const float* topk_w, float* out,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_layer16(L, n);
+    if (rc) return rc;
+    if (n == 0) return GLMMOE_OK;   // no tokens: nothing to compute or write
+    if (!x || !out || !workspace || !topk_ids || !topk_w) return GLMMOE_ERR_ARG;
+    if (reinterpret_cast<uintptr_t>(x) % 16 || reinterpret_cast<uintptr_t>(workspace) % 16)
+        return GLMMOE_ERR_ARG;
+    glmmoe_bf16_ws v;
+    if (carve16(L, n, static_cast<char*>(workspace), &v) > workspace_bytes)
+        return GLMMOE_ERR_WORKSPACE;
+    begin_call();
+    return run_experts16(L, x, n, topk_ids, topk_w, out, v, S(stream));
 }
 
 int glmmoe_profile_enable(int on) {

@@ -1,0 +1,91 @@
+// The two 16-bit number types of the ragged products (grouped.hip, lora.hip):
+// fragments, matrix instructions, conversions, and loads of 8 consecutive values.
+#pragma once
+
+#include "common.hpp"
+
+namespace glmmoe {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
+// Data type codes of the C entries (GLMMOE_F32 / BF16 / F16).
+constexpr int kF32 = 0, kBf16 = 1, kF16 = 2;
+
+struct Bf16 {
+    static constexpr int code = kBf16;
+    static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                       __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack2(float a, float b) { return pack_bf16x2(a, b); }
+    static __device__ __forceinline__ float up(uint32_t h) { return bf16_to_f32(h & 0xffffu); }
+};
+
+struct F16 {
+    static constexpr int code = kF16;
+    static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    // Round to nearest even, as the hardware conversion does.
+    static __device__ __forceinline__ uint32_t pack2(float a, float b) {
+        return __builtin_bit_cast(uint32_t, (f16x2){(_Float16)a, (_Float16)b});
+    }
+    static __device__ __forceinline__ float up(uint32_t h) {
+        return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+    }
+};
+
+// 8 values k .. k + 7 of a row, all inside it. AL: 16-byte aligned.
+template <bool AL, bool NT = false>
+__device__ __forceinline__ u32x4 load8(const uint16_t* row, int k) {
+    if constexpr (AL) {
+        const u32x4* p = reinterpret_cast<const u32x4*>(row + k);
+        if constexpr (NT) return __builtin_nontemporal_load(p);
+        return *p;
+    } else {
+        return *reinterpret_cast<const u32x4_any*>(row + k);
+    }
+}
+
+// The same with zeros from K on. AL: K is a multiple of 8.
+template <bool AL>
+__device__ __forceinline__ u32x4 load8_tail(const uint16_t* row, int k, int K) {
+    if (k + 8 <= K) return load8<AL>(row, k);
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if constexpr (!AL) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (k + i < K) v[i / 2] |= (uint32_t)row[k + i] << (16 * (i & 1));
+    }
+    return v;
+}
+
+// Four consecutive outputs of a row, the first `cnt` of them: one store where VEC.
+template <class T, bool F32>
+__device__ __forceinline__ void store4(void* y, long at, f32x4 v, int cnt, bool vec) {
+    if constexpr (F32) {
+        float* p = static_cast<float*>(y) + at;
+        if (vec) {
+            *reinterpret_cast<f32x4*>(p) = v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < cnt) p[i] = v[i];
+        }
+    } else {
+        uint16_t* p = static_cast<uint16_t*>(y) + at;
+        const u32x2 w = {T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
+        if (vec) {
+            *reinterpret_cast<u32x2*>(p) = w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < cnt) p[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        }
+    }
+}
+
+}  // namespace glmmoe

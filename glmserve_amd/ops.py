@@ -4,11 +4,12 @@ Names, argument order and meaning follow the reference launchers; tensors are
 device tensors and `stream` is a torch.cuda.Stream or None (current stream).
 Unlike the reference (void return, errors printed), failures raise GlmMoeError.
 """
-import torch
-
+import contextlib
 import ctypes
 
-from ._lib import Fp8Layer, Fp8Ws, GlmMoeError, Layer, LayerWs, check, lib
+import torch
+
+from ._lib import Bf16Layer, Bf16Ws, Fp8Layer, Fp8Ws, GlmMoeError, Layer, LayerWs, check, lib
 
 
 def _p(t):
@@ -210,6 +211,153 @@ class FP8MoELayer(_MoELayer):
     _fn = dict(ws_bytes="glmmoe_fp8_layer_workspace_bytes",
                ws_view="glmmoe_fp8_layer_workspace_view", layer="glmmoe_moe_layer_fp8",
                ffn="glmmoe_expert_ffn_fp8")
+
+
+class BF16MoELayer(_MoELayer):
+    """bf16 experts in the checkpoint's layout: gate / up [E, I, H], down [E, H, I], the
+    shared expert's (gate [I, H], up [I, H], down [H, I]) or None, all torch.bfloat16."""
+    _struct = Bf16Layer
+    _view = Bf16Ws
+    _fn = dict(ws_bytes="glmmoe_bf16_layer_workspace_bytes",
+               ws_view="glmmoe_bf16_layer_workspace_view", layer="glmmoe_moe_layer_bf16",
+               ffn="glmmoe_expert_ffn_bf16")
+
+    def __init__(self, hidden, moe_inter, n_experts, topk, router_w, e_bias, gate, up, down,
+                 shared=None, norm_topk=True, routed_scale=2.5):
+        H, I, E = hidden, moe_inter, n_experts
+        self.hidden, self.moe_inter, self.n_experts, self.topk = H, I, E, topk
+        bf = torch.bfloat16
+        if router_w is not None:
+            _need(router_w, bf, E * H, "router_w")
+        if e_bias is not None:
+            _need(e_bias, torch.float32, E, "e_bias")
+        for t, name in ((gate, "gate"), (up, "up"), (down, "down")):
+            _need(t, bf, E * I * H, name)
+        for t in shared or ():
+            _need(t, bf, I * H, "shared")
+        self.keep = [router_w, e_bias, gate, up, down, shared]
+        st = Bf16Layer()
+        st.hidden, st.moe_inter, st.n_experts, st.topk = H, I, E, topk
+        st.norm_topk, st.routed_scale = int(bool(norm_topk)), float(routed_scale)
+        st.router_w, st.e_bias = _p(router_w), _p(e_bias)
+        st.gate, st.up, st.down = _p(gate), _p(up), _p(down)
+        if shared is not None:
+            st.sh_gate, st.sh_up, st.sh_down = (_p(t) for t in shared)
+        self.struct = st
+
+
+# ---- Ragged products on 16-bit weights -------------------------------------------
+
+_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev):
+    """Makes dev the current device for a call (nothing to do where it is)."""
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _need_rows(t, dtypes, rows, cols, name, device=None):
+    """A [>= rows, cols] tensor whose rows are contiguous (any row stride); its row stride."""
+    if (t is None or not t.is_cuda or t.dtype not in dtypes or t.dim() != 2 or t.shape[0] < rows
+            or t.shape[1] != cols or (cols > 1 and t.stride(1) != 1)
+            or (device is not None and t.device != device)):
+        raise GlmMoeError(f"{name}: expected cuda {' / '.join(str(d) for d in dtypes)} with >= {rows} rows of "
+                          f"{cols} contiguous elements" + (f" on {device}" if device else ""))
+    return t.stride(0) if t.shape[0] > 1 else cols
+
+
+def _need_on(t, dtype, numel, name, device):
+    _need(t, dtype, numel, name)
+    if t.device != device:
+        raise GlmMoeError(f"{name}: expected a tensor on {device}")
+
+
+def _stack(w, E, N, K, dtype, name, device):
+    """Element stride between the [N, K] matrices of a [E, N, K] tensor."""
+    if (not w.is_cuda or w.device != device or w.dtype != dtype or tuple(w.shape) != (E, N, K)
+            or (K > 1 and w.stride(2) != 1) or (N > 1 and w.stride(1) != K)):
+        raise GlmMoeError(f"{name}: expected cuda {dtype} [{E}, {N}, {K}] of contiguous matrices on {device}")
+    return w.stride(0) if E > 1 else N * K
+
+
+def _grouped(what, x, ws, expert_offsets, y, row_ids, stream):
+    half = (torch.bfloat16, torch.float16)
+    if x is None or x.dim() != 2 or ws[0].dim() != 3 or y is None or y.dim() != 2:
+        raise GlmMoeError(f"{what}: expected x [rows, K], weights [E, N, K] and an output [rows, N]")
+    dev = x.device
+    E, N, K = ws[0].shape
+    rows = y.shape[0]
+    ldx = _need_rows(x, half, rows if row_ids is None else 0, K, "x")
+    strides = [_stack(w, E, N, K, x.dtype, "w", dev) for w in ws]
+    if len(set(strides)) > 1:
+        raise GlmMoeError(f"{what}: the two weight tensors have different expert strides")
+    ldy = _need_rows(y, (torch.float32, x.dtype), 0, N, "y", dev)
+    _need_on(expert_offsets, torch.int32, E + 1, "expert_offsets", dev)
+    if row_ids is not None:
+        _need_on(row_ids, torch.int32, rows, "row_ids", dev)
+    with _on(dev):
+        check(getattr(lib(), "glmmoe_" + what)(
+            _DTYPE[x.dtype], _p(x), ldx, x.shape[0], _p(row_ids), *[_p(w) for w in ws], strides[0],
+            _p(expert_offsets), E, rows, N, K, _DTYPE[y.dtype], _p(y), ldy, _s(stream)), what)
+
+
+def grouped_linear(x, w, expert_offsets, y, row_ids=None, stream=None):
+    """y[r] = w[e] @ x[row_ids[r]] (x[r] without row_ids) for the rows r in
+    [expert_offsets[e], expert_offsets[e + 1]) of expert e, as moe_dispatch groups them.
+    x [*, K] and w [E, N, K] bf16 or fp16; y [rows, N] of x's type or fp32; rows of x and y,
+    and the matrices of w, may be strided. expert_offsets [E + 1], row_ids [rows] int32.
+    Rows outside the offsets are left as they are."""
+    _grouped("grouped_linear", x, (w,), expert_offsets, y, row_ids, stream)
+
+
+def grouped_gate_up(x, w_gate, w_up, expert_offsets, h, row_ids=None, stream=None):
+    """h[r] = silu(w_gate[e] @ x) * (w_up[e] @ x), x and the rows as grouped_linear takes
+    them; w_gate and w_up [E, N, K] may be the halves of one [E, 2 N, K] tensor."""
+    _grouped("grouped_gate_up", x, (w_gate, w_up), expert_offsets, h, row_ids, stream)
+
+
+def lora_workspace_bytes(n, n_adapters, K, r):
+    return lib().glmmoe_lora_workspace_bytes(n, n_adapters, K, r)
+
+
+def lora_add(x, adapter_ids, A, B, scale, base, y, ranks=None, ws=None, stream=None):
+    """y[t] = base[t] + scale[a] * (B[a] @ (A[a] @ x[t])), a = adapter_ids[t]; tokens whose id
+    is outside [0, n_adapters) get base[t]. x [n, K] fp32 or the adapters' type, A
+    [n_adapters, r, K], B [n_adapters, N, r] bf16 or fp16, scale [n_adapters] fp32 or None;
+    base and y [n, N] fp32 or the adapters' type, the same tensor to add in place. ranks
+    [n_adapters] int32: ranks in use of each adapter. ws: a uint8 tensor of
+    lora_workspace_bytes, else allocated for the call."""
+    half, dev = (torch.bfloat16, torch.float16), x.device
+    if A.dim() != 3 or B.dim() != 3 or A.dtype not in half:
+        raise GlmMoeError("lora_add: expected A [adapters, r, K] and B [adapters, N, r], bf16 or fp16")
+    L, r, K = A.shape
+    N, n = B.shape[1], x.shape[0]
+    _need_on(A, A.dtype, L * r * K, "A", dev)
+    if tuple(B.shape) != (L, N, r):
+        raise GlmMoeError(f"B: expected [{L}, {N}, {r}]")
+    _need_on(B, A.dtype, L * N * r, "B", dev)
+    ldx = _need_rows(x, (torch.float32, A.dtype), n, K, "x")
+    _need_on(adapter_ids, torch.int32, n, "adapter_ids", dev)
+    ldb = _need_rows(base, (torch.float32, A.dtype), n, N, "base", dev)
+    ldy = _need_rows(y, (base.dtype,), n, N, "y", dev)
+    if scale is not None:
+        _need_on(scale, torch.float32, L, "scale", dev)
+    if ranks is not None:
+        _need_on(ranks, torch.int32, L, "ranks", dev)
+    with _on(dev):
+        if ws is None:
+            # On the stream that uses it, so that the allocator keeps it until then.
+            with _HERE if stream is None else torch.cuda.stream(stream):
+                ws = torch.empty(lora_workspace_bytes(n, L, K, r), dtype=torch.uint8, device=dev)
+        else:
+            _need_on(ws, torch.uint8, 0, "ws", dev)
+        check(lib().glmmoe_lora_add(
+            _DTYPE[x.dtype], _p(x), ldx, _p(adapter_ids), n, _DTYPE[A.dtype], _p(A), _p(B), _p(ranks),
+            _p(scale), L, r, K, N, _DTYPE[y.dtype], _p(base), ldb, _p(y), ldy, _p(ws), ws.numel(),
+            _s(stream)), "lora_add")
 
 
 def pack_fp8(w, n_mats, rows, K, out=None, stream=None):

@@ -297,8 +297,123 @@ int glmmoe_expert_ffn_fp8(const glmmoe_fp8_layer* L, const uint16_t* x, int n,
                           const int* topk_ids, const float* topk_w, float* out,
                           void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Ragged products on 16-bit weights ----------------------------------------
+ * Weights stay as a checkpoint stores them, row-major [rows, K], bf16 or fp16;
+ * nothing is packed. `dtype` and the like take these codes: */
+#define GLMMOE_F32 0
+#define GLMMOE_BF16 1
+#define GLMMOE_F16 2
+
+/* Linears grouped by expert: for expert e and its rows r in
+ * [expert_offsets[e], expert_offsets[e + 1])
+ *   y[r, n] = sum_k x[row(r), k] * w[e, n, k],  row(r) = row_ids[r], or r without row_ids
+ * (the products of GLM52Model::moe_mlp, src/model_glm52.cpp:1133-1141, for all the rows
+ * of an expert at once). Sums in fp32, rounded once to y_dtype.
+ *   dtype           GLMMOE_BF16 or GLMMOE_F16, of x and w
+ *   x, ldx, x_rows  [x_rows, K], rows ldx elements apart
+ *   row_ids         [rows] or NULL; a row of x may occur often. A row whose id is outside
+ *                   [0, x_rows) gives zeros
+ *   w, w_stride     expert e's [N, K] matrix at w + e * w_stride elements
+ *   expert_offsets  [E + 1], ascending, as glmmoe_moe_dispatch writes them. Rows before
+ *                   the first and from the last on are left as they are in y; offsets
+ *                   outside [0, rows] are taken as the nearest of the two
+ *   y, y_dtype, ldy [rows, N], rows ldy apart; GLMMOE_F32, or dtype
+ * Any N and K; K, ldx and w_stride multiples of 8 with 16-byte aligned x and w are read
+ * in whole vectors. y must not overlap x. rows == 0 returns GLMMOE_OK. No workspace.
+ * Limits: E <= 4096, rows and x_rows < 2^30, K and N < 2^24. */
+int glmmoe_grouped_linear(int dtype, const void* x, int64_t ldx, int64_t x_rows,
+                          const int* row_ids, const void* w, int64_t w_stride,
+                          const int* expert_offsets, int E, int64_t rows, int64_t N, int64_t K,
+                          int y_dtype, void* y, int64_t ldy, void* stream);
+
+/* Two such products and the experts' activation: h[r, i] = silu(g) * u with
+ * g = x w_gate[e]^T and u = x w_up[e]^T, both [N, K] with w_stride between experts (a
+ * stacked [E, 2 N, K] checkpoint tensor is w_gate = t, w_up = t + N * K, w_stride =
+ * 2 * N * K). g, u and the activation are fp32; one rounding to h_dtype. */
+int glmmoe_grouped_gate_up(int dtype, const void* x, int64_t ldx, int64_t x_rows,
+                           const int* row_ids, const void* w_gate, const void* w_up,
+                           int64_t w_stride, const int* expert_offsets, int E, int64_t rows,
+                           int64_t N, int64_t K, int h_dtype, void* h, int64_t ldh, void* stream);
+
+/* Low-rank adapters of many requests beside a shared projection:
+ *   y[t, :] = base[t, :] + scale[a] * B[a] (A[a] x[t]),  a = adapter_ids[t]
+ * base is the projection's output (glmmoe_ref_gemm_w4a16, _fp8, _q or any other).
+ *   adapter_ids [n]; a token whose id is outside [0, n_adapters) has none: y = base
+ *   x           [n, K], rows ldx apart; GLMMOE_F32, or w_dtype
+ *   A, B        [n_adapters, r, K] and [n_adapters, N, r], GLMMOE_BF16 or GLMMOE_F16
+ *   ranks       [n_adapters] or NULL: adapter a uses its first ranks[a] (0 to r) ranks,
+ *               what A and B hold beyond them is not used
+ *   scale       [n_adapters] fp32 or NULL (1)
+ *   base, y     [n, N], rows ldb and ldy apart; GLMMOE_F32, or w_dtype. y may be base
+ *               (with ldy == ldb) and must not overlap it otherwise
+ * A x stays in fp32 and enters the second product as three bf16 terms, which hold it
+ * exactly; fp32 rows of x enter the first so, too (values below 2^-110 lose their last
+ * bits). One rounding, to y's type. Sums run in a fixed order.
+ * Tokens of a request are expected to be neighbours: 16 to 64 consecutive tokens share
+ * the weights of each adapter that occurs among them.
+ * Workspace: glmmoe_lora_workspace_bytes (A x; 0 for arguments out of range). n == 0
+ * returns GLMMOE_OK. Limits: r <= 256, n < 2^24, K and N < 2^24. */
+size_t glmmoe_lora_workspace_bytes(int n, int n_adapters, int64_t K, int r);
+int glmmoe_lora_add(int x_dtype, const void* x, int64_t ldx, const int* adapter_ids, int n,
+                    int w_dtype, const void* A, const void* B, const int* ranks,
+                    const float* scale, int n_adapters, int r, int64_t K, int64_t N, int y_dtype,
+                    const void* base, int64_t ldb, void* y, int64_t ldy, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* ---- bf16 experts ----------------------------------------------------------
+ * The layer of glmmoe_moe_layer_w4a16 with expert weights in bf16 as a checkpoint
+ * stores them (the reference holds such experts as fp32 and runs them per token,
+ * cuda/kernels.cuh:252-257): router -> dispatch -> grouped gate/up -> grouped down ->
+ * combine with the shared expert. Products are summed in fp32; h = SiLU(gate) * up is
+ * rounded to bf16 for the down product (half the bytes of its input, and the matrix
+ * cores' type); the expert outputs stay fp32 through the combine.
+ * Limits: hidden % 256 == 0, hidden <= 8192, moe_inter % 8 == 0, weights 16-byte
+ * aligned, E <= 512, 1 <= topk <= 8. */
+typedef struct glmmoe_bf16_layer {
+    int hidden;
+    int moe_inter;
+    int n_experts;
+    int topk;
+    int norm_topk;
+    float routed_scale;
+    const uint16_t* router_w;   /* [E, H] */
+    const float* e_bias;        /* [E] fp32 or NULL */
+    const uint16_t* gate;       /* [E, I, H] */
+    const uint16_t* up;         /* [E, I, H] */
+    const uint16_t* down;       /* [E, H, I] */
+    const uint16_t* sh_gate;    /* [I, H] or NULL (no shared expert) */
+    const uint16_t* sh_up;      /* [I, H] */
+    const uint16_t* sh_down;    /* [H, I] */
+} glmmoe_bf16_layer;
+
+typedef struct glmmoe_bf16_ws {
+    float* logits;        /* [n, E] */
+    float* rpart;         /* router chunk partials */
+    int* topk_ids;        /* [n, topk] */
+    float* topk_w;        /* [n, topk] */
+    int* expert_offsets;  /* [E + 2] */
+    int* sorted_token_ids;/* [R], R = n*topk + n with a shared expert */
+    int* sorted_row;      /* [R] */
+    int* inv;             /* [n*topk] */
+    int* tiles;           /* [max_tiles * 4] */
+    int* ntiles;          /* [3] */
+    uint16_t* h;          /* [R, I] bf16 */
+    float* dpart;         /* [R, H] fp32 per-row expert outputs */
+    size_t bytes;
+} glmmoe_bf16_ws;
+
+size_t glmmoe_bf16_layer_workspace_bytes(const glmmoe_bf16_layer* L, int n);
+int glmmoe_bf16_layer_workspace_view(const glmmoe_bf16_layer* L, int n, void* workspace,
+                                     glmmoe_bf16_ws* view);
+/* x: [n, H] bf16; out: [n, H] fp32 (overwritten). */
+int glmmoe_moe_layer_bf16(const glmmoe_bf16_layer* L, const uint16_t* x, int n, float* out,
+                          void* workspace, size_t workspace_bytes, void* stream);
+int glmmoe_expert_ffn_bf16(const glmmoe_bf16_layer* L, const uint16_t* x, int n,
+                           const int* topk_ids, const float* topk_w, float* out,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- Stage timing (diagnostics; no reference counterpart) -----------------
- * While enabled, every layer / expert-FFN call (W4A16 and FP8)
+ * While enabled, every layer / expert-FFN call (W4A16, FP8 and bf16)
  * records a HIP event on its stream before and after each stage, in a ring of
  * GLMMOE_PROF_MAX_CALLS calls (events are created on the first enable; no
  * device memory is allocated). glmmoe_profile_read waits for the recorded
