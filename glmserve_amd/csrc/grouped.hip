@@ -12,35 +12,68 @@
 
 namespace glmmoe {
 
-// Row tile t (tiles of 2^lg rows, in expert order) of the groups off[0 .. E]:
-// its expert, first row and rows; false if there are fewer tiles. Every wave
-// calls it and gets the same answer. Offsets are clamped to [0, rows], so that no
-// tile leaves the rows whatever they hold.
-__device__ __forceinline__ bool find_tile(const int* __restrict__ off, int E, int rows, int lg,
-                                          int t, int& e, int& r0, int& nr) {
-    const int lane = threadIdx.x & 63;
-    const int per = (E + 63) / 64;
-    auto at = [&](int i) { return min(max(off[min(i, E)], 0), rows); };
-    auto tiles = [&](int i) { return i < E ? (max(at(i + 1) - at(i), 0) + (1 << lg) - 1) >> lg : 0; };
-    int sum = 0;
-    for (int j = 0; j < per; ++j) sum += tiles(lane * per + j);
-    int incl = sum;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int v = __shfl_up(incl, d);
-        if (lane >= d) incl += v;
+// Row tiles (2^lg rows at most, in expert order) of the groups off[0 .. E]: how many, and the
+// expert, first row and rows of one. Every wave calls it and gets the same answer. Offsets
+// are clamped to [0, rows], so that no tile leaves the rows whatever they hold.
+struct TileScan {
+    const int* off;
+    int E, rows, lg, per, sum, incl;
+
+    __device__ __forceinline__ int at(int i) const { return min(max(off[min(i, E)], 0), rows); }
+    __device__ __forceinline__ int tiles(int i) const {
+        return i < E ? (max(at(i + 1) - at(i), 0) + (1 << lg) - 1) >> lg : 0;
     }
-    const uint64_t past = __ballot(incl > t);
-    if (past == 0) return false;
-    const int first = __builtin_ctzll(past);
-    int rest = t - __builtin_amdgcn_readlane(incl - sum, first);
-    e = first * per;
-    for (int j = 1, c = tiles(e); j < per && rest >= c; ++j, c = tiles(++e)) rest -= c;
-    e = __builtin_amdgcn_readfirstlane(e);
-    rest = __builtin_amdgcn_readfirstlane(rest);
-    r0 = __builtin_amdgcn_readfirstlane(at(e)) + (rest << lg);
-    nr = min(__builtin_amdgcn_readfirstlane(at(e + 1)) - r0, 1 << lg);
-    return e < E && nr > 0;
+    __device__ __forceinline__ TileScan(const int* o, int E_, int rows_, int lg_)
+        : off(o), E(E_), rows(rows_), lg(lg_), per((E_ + 63) / 64), sum(0) {
+        const int lane = threadIdx.x & 63;
+        for (int j = 0; j < per; ++j) sum += tiles(lane * per + j);
+        incl = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int v = __shfl_up(incl, d);
+            if (lane >= d) incl += v;
+        }
+    }
+    __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(incl, 63); }
+    __device__ __forceinline__ bool find(int t, int& e, int& r0, int& nr) const {
+        const uint64_t past = __ballot(incl > t);
+        if (past == 0) return false;
+        const int first = __builtin_ctzll(past);
+        int rest = t - __builtin_amdgcn_readlane(incl - sum, first);
+        e = first * per;
+        for (int j = 1, c = tiles(e); j < per && rest >= c; ++j, c = tiles(++e)) rest -= c;
+        e = __builtin_amdgcn_readfirstlane(e);
+        rest = __builtin_amdgcn_readfirstlane(rest);
+        r0 = __builtin_amdgcn_readfirstlane(at(e)) + (rest << lg);
+        nr = min(__builtin_amdgcn_readfirstlane(at(e + 1)) - r0, 1 << lg);
+        return e < E && nr > 0;
+    }
+};
+
+// The item of workgroup `id` among `total`: workgroups go round-robin to the 8 XCDs (id % 8), and
+// each XCD takes a contiguous run of items, so that neighbours share its L2. -1: none left.
+__device__ __forceinline__ long xcd_item(long id, long total) {
+    const long q = total / 8, rem = total % 8, x = id % 8, i = id / 8;
+    if (i >= q + (x < rem)) return -1;
+    return x * q + min(x, rem) + i;
+}
+
+// This workgroup's (tile, block of columns), columns fastest; false if it has none.
+__device__ __forceinline__ bool find_item(const GroupedArgs& a, int lg, int& e, int& r0, int& nr,
+                                          int& col) {
+    if (a.off) {
+        const TileScan scan(a.off, a.E, a.rows, lg);
+        const long item = xcd_item(blockIdx.x, (long)scan.total() * a.ntn);
+        if (item < 0) return false;
+        col = (int)(item % a.ntn);
+        return scan.find((int)(item / a.ntn), e, r0, nr);
+    }
+    const long item = xcd_item(blockIdx.x, (long)min(a.ntiles[0], a.max_tiles) * a.ntn);
+    if (item < 0) return false;
+    col = (int)(item % a.ntn);
+    const int* t = a.tiles + 4 * (item / a.ntn);
+    e = t[0], r0 = t[1], nr = t[2];
+    return true;
 }
 
 // Few rows per expert: the weights are streamed once and bound the time.
@@ -58,17 +91,11 @@ __global__ __launch_bounds__(64 * kStreamWaves) void grp_stream_kernel(GroupedAr
     constexpr int M = DUAL ? 2 : 1, LG = TB == 1 ? 4 : TB == 2 ? 5 : 6, KC = 32 * KS;
     __shared__ f32x4 red[kStreamWaves][M * NB * TB][64];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-    int e, r0, nr;
-    const int tile = (int)(blockIdx.x / a.ntn);
-    if (a.off) {
-        if (!find_tile(a.off, a.E, a.rows, LG, tile, e, r0, nr)) return;
-    } else {
-        if (tile >= a.ntiles[0]) return;
-        e = a.tiles[4 * tile], r0 = a.tiles[4 * tile + 1], nr = a.tiles[4 * tile + 2];
-    }
+    int e, r0, nr, col;
+    if (!find_item(a, LG, e, r0, nr, col)) return;
     const uint16_t *w0 = a.w0 + (long)e * a.w_stride, *w1 = a.w1 + (long)e * a.w_stride;
     if (e == a.E) w0 = a.s0, w1 = a.s1;
-    const int n0 = (int)(blockIdx.x % a.ntn) * 16 * NB;
+    const int n0 = col * 16 * NB;
     const int K = a.K;
 
     const uint16_t* xp[TB];
@@ -188,16 +215,177 @@ __global__ __launch_bounds__(64 * kStreamWaves) void grp_stream_kernel(GroupedAr
     }
 }
 
+// Many rows per expert: tiles of up to 256 rows x 256 rows of W (128 features of both
+// matrices where DUAL), 64 of K per step, two steps' operands in LDS.
+//
+// 8 waves, 2 along the rows x 4 along W: wave (wr, wc) has the 16-row blocks wr, wr + 2, ... of
+// the tile (so that a tile of few rows keeps both wave rows busy) and 64 rows of W. A row of a
+// step is 128 B in LDS, its 16-byte chunk c at slot c ^ (row / 2 % 8): the 16 rows that a
+// fragment read touches at one chunk fall on 16 different groups of banks. Whole rows go
+// straight from memory to LDS, 8 to an instruction. A step has two 32-K halves of one or two row halves
+// each ("phases" of 16 MFMAs); the next phase's fragments are read before this phase's products,
+// and the one barrier of a step stands before its last phase: behind it the next step is complete
+// and the step's own half of LDS is free for the step after that.
+constexpr int kTileWaves = 8, kTileN = 256, kTileK = 64;
+constexpr int kTileHalf = 256 * 128;              // LDS bytes of one operand of a step
+constexpr int kTileLds = 4 * kTileHalf;
+__device__ const u32x4 grp_zero = {0u, 0u, 0u, 0u};
+
+// 64 lanes x 16 B from memory to LDS at base + 16 * lane, without the compiler's knowledge: it
+// would have every LDS read wait for all of them.
+__device__ __forceinline__ void copy16(const void* g, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n s_nop 0\n global_load_lds_dwordx4 %0, off"
+                 :: "v"(g), "s"(lds) : "memory");
+}
+
+template <class T, bool DUAL, bool AL, bool F32>
+struct TileRun {
+    const GroupedArgs& a;
+    char* lds;
+    int e, r0, nr, col, lane, wv;
+
+    // MB: 16-row blocks per wave row.
+    template <int MB>
+    __device__ __forceinline__ void run() {
+        constexpr int MH = MB < 4 ? MB : 4, NP = MB / MH, PH = 2 * NP, CA = MB / 2;
+        const int r = lane & 15, q = lane >> 4, wr = wv >> 2, wc = wv & 3;
+        const int K = a.K, steps = (K + kTileK - 1) / kTileK;
+        const uint16_t *w0 = a.w0 + (long)e * a.w_stride, *w1 = a.w1 + (long)e * a.w_stride;
+        if (e == a.E) w0 = a.s0, w1 = a.s1;
+        const int f0 = col * (DUAL ? kTileN / 2 : kTileN);
+
+        // What this lane copies: chunk `c8` of rows (8 i + wv) * 8 + lane / 8.
+        const int cr = wv * 8 + (lane >> 3), c8 = ((lane & 7) ^ (cr >> 1 & 7)) * 8;
+        const uint16_t *pa[CA], *pb[4];
+#pragma unroll
+        for (int i = 0; i < CA; ++i) {
+            const int j = 64 * i + cr, rr = j < nr ? r0 + j : r0;
+            const int id = a.row_ids ? a.row_ids[rr] : rr;
+            pa[i] = a.x + (id >= 0 && id < a.x_rows ? (long)id : 0) * a.ldx;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = 64 * i + cr;              // row of W in the tile: 64 to a wave column
+            const int n = DUAL ? f0 + (j >> 6) * 32 + (j & 31) : f0 + j;
+            pb[i] = (DUAL && (j & 32) ? w1 : w0) + (long)min(n, a.N - 1) * K;
+        }
+        const uint32_t la = lds_addr(lds);
+        auto fetch = [&](int s) {
+            const uint32_t at = la + (s & 1) * 2 * kTileHalf + wv * 1024;
+            const int k = s * kTileK + c8;
+            const bool in = k < K;                  // K % 8 == 0: a chunk is inside or not
+#pragma unroll
+            for (int i = 0; i < CA; ++i)
+                copy16(in ? static_cast<const void*>(pa[i] + k) : &grp_zero, at + i * 8192);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                copy16(in ? static_cast<const void*>(pb[i] + k) : &grp_zero, at + kTileHalf + i * 8192);
+        };
+        auto frag = [&](int buf, int operand, int row, int kk) {
+            const int c = (kk * 4 + q) ^ (row >> 1 & 7);
+            return *reinterpret_cast<const u32x4*>(lds + buf * 2 * kTileHalf + operand * kTileHalf +
+                                                   row * 128 + c * 16);
+        };
+
+        f32x4 acc[MB][4];
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) acc[m][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        u32x4 fa[2][MH], fb[2][4];
+        auto read = [&](int buf, int p) {           // phase p: half p / NP of K, rows p % NP
+            const int kk = p / NP, h = p % NP;
+#pragma unroll
+            for (int m = 0; m < MH; ++m)
+                fa[p & 1][m] = frag(buf, 0, ((h * MH + m) * 2 + wr) * 16 + r, kk);
+            if (h == 0)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) fb[kk][n] = frag(buf, 1, wc * 64 + n * 16 + r, kk);
+        };
+
+        fetch(0);
+        if (steps > 1) {
+            fetch(1);
+            asm volatile("s_waitcnt vmcnt(%0)" :: "n"(CA + 4) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        asm volatile("s_barrier" ::: "memory");
+        read(0, 0);
+        for (int s = 0; s < steps; ++s) {
+            const int buf = s & 1;
+#pragma unroll
+            for (int p = 0; p < PH; ++p) {
+                if (p + 1 < PH) {
+                    read(buf, p + 1);
+                } else if (s + 1 < steps) {
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n s_barrier" ::: "memory");
+                    read(buf ^ 1, 0);
+                    if (s + 2 < steps) fetch(s + 2);
+                }
+                const int kk = p / NP, h = p % NP;
+#pragma unroll
+                for (int m = 0; m < MH; ++m)
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+                        acc[h * MH + m][n] = T::mma(fb[kk][n], fa[p & 1][m], acc[h * MH + m][n]);
+            }
+        }
+
+        // A lane holds four neighbouring outputs of row `lane % 16` of each block.
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            const int j = (m * 2 + wr) * 16 + r;
+            if (j >= nr) continue;
+            const int id = a.row_ids ? a.row_ids[r0 + j] : 0;
+            const bool ok = !a.row_ids || (id >= 0 && id < a.x_rows);
+#pragma unroll
+            for (int n = 0; n < (DUAL ? 2 : 4); ++n) {
+                f32x4 v = acc[m][n];
+                if constexpr (DUAL) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) v[c] = silu_fast(v[c]) * acc[m][n + 2][c];
+                }
+                if (!ok) v = (f32x4){0.f, 0.f, 0.f, 0.f};
+                const int f = f0 + wc * (DUAL ? 32 : 64) + 16 * n + 4 * q;
+                if (f < a.N)
+                    store4<T, F32>(a.y, (long)(r0 + j) * a.ldy + f, v, a.N - f, a.vec && f + 4 <= a.N);
+            }
+        }
+    }
+};
+
+template <class T, bool DUAL, bool AL, bool F32>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void grp_tile_kernel(GroupedArgs a) {
+    __shared__ __align__(16) char lds[kTileLds];
+    TileRun<T, DUAL, AL, F32> t{a, lds, 0, 0, 0, 0, (int)(threadIdx.x & 63),
+                                __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)};
+    if (!find_item(a, 8, t.e, t.r0, t.nr, t.col)) return;
+    if (t.nr <= 64) t.template run<2>();
+    else if (t.nr <= 128) t.template run<4>();
+    else t.template run<8>();
+}
+
 int grouped_tile_rows(long rows, int E) {
     const long groups = E < rows ? E : rows;
     const long mean = (rows + groups - 1) / groups;
-    return mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
+    return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 48 ? 64 : 256;
 }
 
 template <class T, bool DUAL, bool AL, bool F32>
 static int run_stream(const GroupedArgs& a0, hipStream_t s) {
     GroupedArgs a = a0;
-    const int tb = a.off ? grouped_tile_rows(a.rows, a.E) / 16 : a.tb;
+    int tb = a.off ? grouped_tile_rows(a.rows, a.E) / 16 : a.tb;
+    if (AL && tb == 16) {
+        const int w = DUAL ? kTileN / 2 : kTileN;
+        a.ntn = (a.N + w - 1) / w;
+        const long items = (a.off ? (long)a.rows / 256 + (a.E < a.rows ? a.E : a.rows) : a.max_tiles) * a.ntn;
+        if (items >= (1L << 31)) return -2;
+        hipLaunchKernelGGL((grp_tile_kernel<T, DUAL, AL, F32>), dim3((unsigned)items),
+                           dim3(64 * kTileWaves), 0, s, a);
+        return hipGetLastError() == hipSuccess ? 0 : -4;
+    }
+    if (tb > 4) tb = 4;
     constexpr int NB = DUAL ? 1 : 2;
     a.ntn = (a.N + 16 * NB - 1) / (16 * NB);
     const long tiles = a.off ? (long)a.rows / (16 * tb) + (a.E < a.rows ? a.E : a.rows) : a.max_tiles;
