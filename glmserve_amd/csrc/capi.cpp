@@ -169,16 +169,11 @@ int check_layer16(const glmmoe_bf16_layer* L, int n) {
 
 inline bool has_shared(const glmmoe_bf16_layer* L) { return L->sh_gate != nullptr; }
 
-// Rows of a tile of the layer's grouped products.
-int tile_rows16(const glmmoe_bf16_layer* L, int n) {
-    return grouped_tile_rows((long)n * L->topk, L->n_experts);
-}
-
 size_t carve16(const glmmoe_bf16_layer* L, int n, char* base, glmmoe_bf16_ws* v) {
     const int H = L->hidden, I = L->moe_inter, E = L->n_experts, k = L->topk;
     const size_t nk = (size_t)n * k;
     const size_t R = nk + (has_shared(L) ? (size_t)n : 0);
-    const size_t mt = n ? (size_t)max_tiles_for(n, k, E, has_shared(L), tile_rows16(L, n)) : 0;
+    const size_t mt = (size_t)max_tiles_for(n, k, E, has_shared(L), kBigRows);
     size_t off = 0;
     auto take = [&](size_t bytes) -> char* {
         char* p = base ? base + off : nullptr;
@@ -304,25 +299,22 @@ int run_experts8(const glmmoe_fp8_layer* L, const uint16_t* x, int n, const int*
     return GLMMOE_OK;
 }
 
-// bf16: dispatch, the two grouped products on the dispatch's tiles, the combine.
+// bf16: dispatch, the two grouped products on the dispatch's offsets (they make their own
+// tiles; the shared expert's rows are one more group), the combine.
 int run_experts16(const glmmoe_bf16_layer* L, const uint16_t* x, int n, const int* ids,
                   const float* w, float* out, const glmmoe_bf16_ws& v, hipStream_t s,
                   bool dispatched = false) {
     const int H = L->hidden, I = L->moe_inter, E = L->n_experts, k = L->topk;
     const int sh = has_shared(L) ? 1 : 0;
-    const int T = tile_rows16(L, n);
     mark(GLMMOE_STAGE_DISPATCH, s);
     int rc = dispatched ? 0
                         : launch_dispatch(ids, n, k, E, v.expert_offsets, v.sorted_token_ids,
-                                          v.sorted_row, v.inv, v.tiles, v.ntiles, T, sh, 1, s,
-                                          dispatch_scratch(v.rpart, L, n), 0);
+                                          v.sorted_row, v.inv, v.tiles, v.ntiles, kBigRows, sh, 1,
+                                          s, dispatch_scratch(v.rpart, L, n), 0);
     if (rc) return rc;
     GroupedArgs a{};
-    a.tiles = v.tiles, a.ntiles = v.ntiles;
-    a.max_tiles = max_tiles_for(n, k, E, sh, T);
-    a.tb = T / 16;
-    a.E = E;
-    a.rows = n * (k + sh);
+    a.off = v.expert_offsets, a.E = E, a.rows = n * k;
+    a.sh_row = n * k, a.sh_rows = sh * n;
     a.x = x, a.ldx = H, a.x_rows = n, a.row_ids = v.sorted_token_ids;
     a.w0 = L->gate, a.w1 = L->up, a.w_stride = (long)I * H;
     a.s0 = L->sh_gate, a.s1 = L->sh_up;
@@ -331,7 +323,7 @@ int run_experts16(const glmmoe_bf16_layer* L, const uint16_t* x, int n, const in
     mark(GLMMOE_STAGE_GATE_UP, s);
     rc = launch_grouped(a, GLMMOE_BF16, false, s);
     if (rc) return rc;
-    a.x = v.h, a.ldx = I, a.x_rows = a.rows, a.row_ids = nullptr;
+    a.x = v.h, a.ldx = I, a.x_rows = n * (k + sh), a.row_ids = nullptr;
     a.w0 = L->down, a.w1 = nullptr;
     a.s0 = L->sh_down, a.s1 = nullptr;
     a.N = H, a.K = I;
@@ -659,7 +651,7 @@ int glmmoe_moe_layer_bf16(const glmmoe_bf16_layer* L, const uint16_t* x, int n, 
     begin_call();
     mark(GLMMOE_STAGE_ROUTER_LOGITS, s);
     const DispOut disp{v.expert_offsets, v.sorted_token_ids, v.sorted_row, v.inv,
-                       reinterpret_cast<int4*>(v.tiles), v.ntiles, tile_rows16(L, n),
+                       reinterpret_cast<int4*>(v.tiles), v.ntiles, kBigRows,
                        has_shared(L) ? 1 : 0, 1, 0, nullptr, 0};
     bool dispatched = false;
     rc = launch_router_select(x, L->router_w, L->e_bias, n, L->hidden, L->n_experts, L->topk,

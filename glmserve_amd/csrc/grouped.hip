@@ -12,41 +12,75 @@
 
 namespace glmmoe {
 
-// Row tiles (2^lg rows at most, in expert order) of the groups off[0 .. E]: how many, and the
-// expert, first row and rows of one. Every wave calls it and gets the same answer. Offsets
-// are clamped to [0, rows], so that no tile leaves the rows whatever they hold.
+// Row tiles (2^lg rows at most) of the groups off[0 .. E], and of group E, the shared expert's
+// rows, where there is one: large tiles (more than 2^lg / 2 rows) in expert order, then small ones. Every
+// wave calls it and gets the same answer. Offsets are clamped to [0, rows], so that no tile
+// leaves the rows whatever they hold. Lane i looks after `per` consecutive experts.
 struct TileScan {
-    const int* off;
-    int E, rows, lg, per, sum, incl;
+    const GroupedArgs& a;
+    int lg, per;
+    int o[10];                                      // per <= 9: the lane's offsets
+    int nbig, nsmall, ibig, ismall;                 // the lane's tiles, and up to and with its
 
-    __device__ __forceinline__ int at(int i) const { return min(max(off[min(i, E)], 0), rows); }
-    __device__ __forceinline__ int tiles(int i) const {
-        return i < E ? (max(at(i + 1) - at(i), 0) + (1 << lg) - 1) >> lg : 0;
-    }
-    __device__ __forceinline__ TileScan(const int* o, int E_, int rows_, int lg_)
-        : off(o), E(E_), rows(rows_), lg(lg_), per((E_ + 63) / 64), sum(0) {
-        const int lane = threadIdx.x & 63;
-        for (int j = 0; j < per; ++j) sum += tiles(lane * per + j);
-        incl = sum;
+    __device__ __forceinline__ int at(int i) const { return min(max(a.off[min(i, a.E)], 0), a.rows); }
+    // f(expert, first row, rows) for the lane's experts.
+    template <class F>
+    __device__ __forceinline__ void each(F&& f) const {
+        const int e0 = (threadIdx.x & 63) * per;
+        auto one = [&](int e, int lo, int hi) {
+            if (e == a.E) lo = a.sh_row, hi = a.sh_row + a.sh_rows;
+            f(e, lo, max(hi - lo, 0));
+        };
+        if (per <= 9) {
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int v = __shfl_up(incl, d);
-            if (lane >= d) incl += v;
+            for (int j = 0; j < 9; ++j)
+                if (j < per) one(e0 + j, o[j], o[j + 1]);
+        } else {
+            for (int j = 0; j < per; ++j) one(e0 + j, at(e0 + j), at(e0 + j + 1));
         }
     }
-    __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(incl, 63); }
-    __device__ __forceinline__ bool find(int t, int& e, int& r0, int& nr) const {
+    __device__ __forceinline__ int big(int n) const {
+        return (n >> lg) + ((n & ((1 << lg) - 1)) > 1 << (lg - 1));
+    }
+    __device__ __forceinline__ int small(int n) const {
+        const int rest = n & ((1 << lg) - 1);
+        return rest > 0 && rest <= 1 << (lg - 1);
+    }
+    __device__ __forceinline__ TileScan(const GroupedArgs& a_, int lg_)
+        : a(a_), lg(lg_), per((a_.E + 64) / 64), nbig(0), nsmall(0) {
+        const int lane = threadIdx.x & 63;
+        if (per <= 9) {
+#pragma unroll
+            for (int j = 0; j < 10; ++j)
+                if (j <= per) o[j] = at(lane * per + j);
+        }
+        each([&](int, int, int n) { nbig += big(n), nsmall += small(n); });
+        ibig = nbig, ismall = nsmall;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int u = __shfl_up(ibig, d), v = __shfl_up(ismall, d);
+            if (lane >= d) ibig += u, ismall += v;
+        }
+    }
+    // Tile t of a class, found by the lane that has it.
+    __device__ __forceinline__ bool find(bool large, int t, int& e, int& r0, int& nr) const {
+        const int mine = large ? nbig : nsmall, incl = large ? ibig : ismall;
         const uint64_t past = __ballot(incl > t);
         if (past == 0) return false;
         const int first = __builtin_ctzll(past);
-        int rest = t - __builtin_amdgcn_readlane(incl - sum, first);
-        e = first * per;
-        for (int j = 1, c = tiles(e); j < per && rest >= c; ++j, c = tiles(++e)) rest -= c;
-        e = __builtin_amdgcn_readfirstlane(e);
-        rest = __builtin_amdgcn_readfirstlane(rest);
-        r0 = __builtin_amdgcn_readfirstlane(at(e)) + (rest << lg);
-        nr = min(__builtin_amdgcn_readfirstlane(at(e + 1)) - r0, 1 << lg);
-        return e < E && nr > 0;
+        int rest = t - (incl - mine), ee = -1, rr = 0, nn = 0;
+        each([&](int x, int lo, int n) {
+            const int c = large ? big(n) : small(n);
+            if (rest >= 0 && rest < c) {
+                const int skip = (large ? rest : n >> lg) << lg;
+                ee = x, rr = lo + skip, nn = min(n - skip, 1 << lg);
+            }
+            rest -= c;
+        });
+        e = __builtin_amdgcn_readlane(ee, first);
+        r0 = __builtin_amdgcn_readlane(rr, first);
+        nr = __builtin_amdgcn_readlane(nn, first);
+        return e >= 0 && nr > 0;
     }
 };
 
@@ -58,22 +92,27 @@ __device__ __forceinline__ long xcd_item(long id, long total) {
     return x * q + min(x, rem) + i;
 }
 
-// This workgroup's (tile, block of columns), columns fastest; false if it has none.
+// This workgroup's (tile, block of columns), columns fastest; false if it has none. The large
+// tiles of all experts come before the small ones, each class spread evenly over the XCDs: 16384
+// rows of 16 experts (four large tiles each, half of them with a few rows more) take two rounds of
+// large items and a short one instead of three, 485 -> 410 us.
 __device__ __forceinline__ bool find_item(const GroupedArgs& a, int lg, int& e, int& r0, int& nr,
                                           int& col) {
-    if (a.off) {
-        const TileScan scan(a.off, a.E, a.rows, lg);
-        const long item = xcd_item(blockIdx.x, (long)scan.total() * a.ntn);
-        if (item < 0) return false;
-        col = (int)(item % a.ntn);
-        return scan.find((int)(item / a.ntn), e, r0, nr);
-    }
-    const long item = xcd_item(blockIdx.x, (long)min(a.ntiles[0], a.max_tiles) * a.ntn);
+    const TileScan scan(a, lg);
+    long id = blockIdx.x;
+    const long big = (long)__builtin_amdgcn_readlane(scan.ibig, 63) * a.ntn;
+    const bool large = id < (big + 7) / 8 * 8;
+    if (!large) id -= (big + 7) / 8 * 8;
+    const long item = xcd_item(id, large ? big : (long)__builtin_amdgcn_readlane(scan.ismall, 63) * a.ntn);
     if (item < 0) return false;
     col = (int)(item % a.ntn);
-    const int* t = a.tiles + 4 * (item / a.ntn);
-    e = t[0], r0 = t[1], nr = t[2];
-    return true;
+    return scan.find(large, (int)(item / a.ntn), e, r0, nr);
+}
+// Workgroups for tiles of `rows` rows: as many as there may be tiles, and what the classes'
+// rounding to 8 adds.
+static long grid_items(const GroupedArgs& a, int tile_rows) {
+    const long groups = a.E + (a.sh_rows > 0), rows = (long)a.rows + a.sh_rows;
+    return (rows / tile_rows + (groups < rows ? groups : rows)) * a.ntn + 16;
 }
 
 // Few rows per expert: the weights are streamed once and bound the time.
@@ -215,20 +254,18 @@ __global__ __launch_bounds__(64 * kStreamWaves) void grp_stream_kernel(GroupedAr
     }
 }
 
-// Many rows per expert: tiles of up to 256 rows x 256 rows of W (128 features of both
-// matrices where DUAL), 64 of K per step, two steps' operands in LDS.
+// Tiles of rows x TN rows of W (TN / 2 features of both matrices where DUAL), 64 of K per
+// step, D steps in LDS.
 //
-// 8 waves, 2 along the rows x 4 along W: wave (wr, wc) has the 16-row blocks wr, wr + 2, ... of
-// the tile (so that a tile of few rows keeps both wave rows busy) and 64 rows of W. A row of a
-// step is 128 B in LDS, its 16-byte chunk c at slot c ^ (row / 2 % 8): the 16 rows that a
-// fragment read touches at one chunk fall on 16 different groups of banks. Whole rows go
-// straight from memory to LDS, 8 to an instruction. A step has two 32-K halves of one or two row halves
-// each ("phases" of 16 MFMAs); the next phase's fragments are read before this phase's products,
-// and the one barrier of a step stands before its last phase: behind it the next step is complete
-// and the step's own half of LDS is free for the step after that.
-constexpr int kTileWaves = 8, kTileN = 256, kTileK = 64;
-constexpr int kTileHalf = 256 * 128;              // LDS bytes of one operand of a step
-constexpr int kTileLds = 4 * kTileHalf;
+// Waves stand WR along the rows x WC along W: wave (wr, wc) has MB 16-row blocks wr, wr + WR, ...
+// of the tile (so that a tile of few rows keeps every wave busy) and NB blocks of 16 rows of W. A
+// row of a step is 128 B in LDS, its 16-byte chunk c at slot c ^ (row / 2 % 8): the 16 rows that
+// a fragment read touches at one chunk fall on 16 different groups of banks. Rows go straight
+// from memory to LDS, 8 whole rows to an instruction (steps of 32 K, 64 B a row, streamed W at
+// 5.6 instead of 6.3 TB/s). Fragments are read one phase (up to 16 products) ahead; the one
+// barrier of a step stands before its last phase: behind it the next step is complete and this
+// step's LDS is free for the step D later.
+constexpr int kTileK = 64;
 __device__ const u32x4 grp_zero = {0u, 0u, 0u, 0u};
 
 // 64 lanes x 16 B from memory to LDS at base + 16 * lane, without the compiler's knowledge: it
@@ -238,116 +275,160 @@ __device__ __forceinline__ void copy16(const void* g, uint32_t lds) {
                  :: "v"(g), "s"(lds) : "memory");
 }
 
-template <class T, bool DUAL, bool AL, bool F32>
+template <class T, bool DUAL, bool F32, int WR, int WC, int NB, int LDS>
 struct TileRun {
+    static constexpr int W = WR * WC, TN = WC * NB * 16;
     const GroupedArgs& a;
     char* lds;
     int e, r0, nr, col, lane, wv;
 
-    // MB: 16-row blocks per wave row.
     template <int MB>
     __device__ __forceinline__ void run() {
-        constexpr int MH = MB < 4 ? MB : 4, NP = MB / MH, PH = 2 * NP, CA = MB / 2;
-        const int r = lane & 15, q = lane >> 4, wr = wv >> 2, wc = wv & 3;
+        constexpr int NP = MB > 4 ? 2 : 1, MH = (MB + NP - 1) / NP, PH = 2 * NP;
+        constexpr int NA = MB * WR * 2, CA = (NA + W - 1) / W, CB = TN / 8 / W, BOFF = NA * 1024,
+                      STAGE = (NA + TN / 8) * 1024, D0 = LDS / STAGE, D = D0 < 8 ? D0 : 8;
+        static_assert(D >= 2 && CB * W * 8 == TN, "two steps, whole instructions");
+        const int r = lane & 15, q = lane >> 4, wr = wv / WC, wc = wv % WC;
         const int K = a.K, steps = (K + kTileK - 1) / kTileK;
         const uint16_t *w0 = a.w0 + (long)e * a.w_stride, *w1 = a.w1 + (long)e * a.w_stride;
         if (e == a.E) w0 = a.s0, w1 = a.s1;
-        const int f0 = col * (DUAL ? kTileN / 2 : kTileN);
+        const int f0 = col * (DUAL ? TN / 2 : TN);
 
-        // What this lane copies: chunk `c8` of rows (8 i + wv) * 8 + lane / 8.
-        const int cr = wv * 8 + (lane >> 3), c8 = ((lane & 7) ^ (cr >> 1 & 7)) * 8;
-        const uint16_t *pa[CA], *pb[4];
-#pragma unroll
-        for (int i = 0; i < CA; ++i) {
-            const int j = 64 * i + cr, rr = j < nr ? r0 + j : r0;
-            const int id = a.row_ids ? a.row_ids[rr] : rr;
-            pa[i] = a.x + (id >= 0 && id < a.x_rows ? (long)id : 0) * a.ldx;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int j = 64 * i + cr;              // row of W in the tile: 64 to a wave column
-            const int n = DUAL ? f0 + (j >> 6) * 32 + (j & 31) : f0 + j;
-            pb[i] = (DUAL && (j & 32) ? w1 : w0) + (long)min(n, a.N - 1) * K;
-        }
+        // What this lane copies: chunk c8 of row lane / 8 of pieces of 8 rows. Of x, piece
+        // W i + wv of the NA (waves past the last one repeat a piece).
+        const int cr = lane >> 3;
+        const uint16_t *pa[CA], *pb[CB];
+        int at[CA], ka[CA], kb[CB];
         const uint32_t la = lds_addr(lds);
-        auto fetch = [&](int s) {
-            const uint32_t at = la + (s & 1) * 2 * kTileHalf + wv * 1024;
-            const int k = s * kTileK + c8;
-            const bool in = k < K;                  // K % 8 == 0: a chunk is inside or not
+        // Chunks from K on are zeros (K % 8 == 0: a chunk is inside or not).
+        auto fetch_w = [&](int s, uint32_t stage) {
+            const int k = s * kTileK;
+            const bool whole = k + kTileK <= K;
+#pragma unroll
+            for (int i = 0; i < CB; ++i)
+                copy16(whole || k + kb[i] < K ? static_cast<const void*>(pb[i] + k) : &grp_zero,
+                       la + stage + BOFF + (W * i + wv) * 1024);
+        };
+        auto fetch_x = [&](int s, uint32_t stage) {
+            const int k = s * kTileK;
+            const bool whole = k + kTileK <= K;
 #pragma unroll
             for (int i = 0; i < CA; ++i)
-                copy16(in ? static_cast<const void*>(pa[i] + k) : &grp_zero, at + i * 8192);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                copy16(in ? static_cast<const void*>(pb[i] + k) : &grp_zero, at + kTileHalf + i * 8192);
+                copy16(whole || k + ka[i] < K ? static_cast<const void*>(pa[i] + k) : &grp_zero,
+                       la + stage + at[i] * 1024);
         };
-        auto frag = [&](int buf, int operand, int row, int kk) {
-            const int c = (kk * 4 + q) ^ (row >> 1 & 7);
-            return *reinterpret_cast<const u32x4*>(lds + buf * 2 * kTileHalf + operand * kTileHalf +
-                                                   row * 128 + c * 16);
+        // The first steps' W is on its way while the rows of x are looked up.
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+            const int j = 8 * (W * i + wv) + cr;    // row of W in the tile; a wave's are gate, then up
+            const int n = DUAL ? f0 + j / (16 * NB) * 8 * NB + j % (8 * NB) : f0 + j;
+            kb[i] = ((lane & 7) ^ (j >> 1 & 7)) * 8;
+            pb[i] = (DUAL && j % (16 * NB) >= 8 * NB ? w1 : w0) + (long)min(n, a.N - 1) * K + kb[i];
+        }
+        int ids[CA];
+#pragma unroll
+        for (int i = 0; i < CA; ++i) {
+            at[i] = (W * i + wv) % NA;
+            const int j = 8 * at[i] + cr, rr = j < nr ? r0 + j : r0;
+            ids[i] = a.row_ids ? a.row_ids[rr] : rr;
+            ka[i] = ((lane & 7) ^ (j >> 1 & 7)) * 8;
+        }
+#pragma unroll
+        for (int s = 0; s < D - 1; ++s)
+            if (s < steps) fetch_w(s, s * STAGE);
+#pragma unroll
+        for (int i = 0; i < CA; ++i)
+            pa[i] = a.x + (ids[i] >= 0 && ids[i] < a.x_rows ? (long)ids[i] : 0) * a.ldx + ka[i];
+#pragma unroll
+        for (int s = 0; s < D - 1; ++s)
+            if (s < steps) fetch_x(s, s * STAGE);
+        auto fetch = [&](int s, uint32_t stage) {
+            const int k = s * kTileK;
+            if (k + kTileK <= K) {
+#pragma unroll
+                for (int i = 0; i < CB; ++i) copy16(pb[i] + k, la + stage + BOFF + (W * i + wv) * 1024);
+#pragma unroll
+                for (int i = 0; i < CA; ++i) copy16(pa[i] + k, la + stage + at[i] * 1024);
+            } else {
+                fetch_w(s, stage);
+                fetch_x(s, stage);
+            }
         };
 
-        f32x4 acc[MB][4];
+        f32x4 acc[MB][NB];
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
-            for (int n = 0; n < 4; ++n) acc[m][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        u32x4 fa[2][MH], fb[2][4];
-        auto read = [&](int buf, int p) {           // phase p: half p / NP of K, rows p % NP
-            const int kk = p / NP, h = p % NP;
+            for (int n = 0; n < NB; ++n) acc[m][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        u32x4 fa[2][MH], fb[2][NB];
+        // (Row / 2) % 8 is that of r in every block of 16 rows.
+        const char* ra = lds + (wr * 16 + r) * 128;
+        const char* rb = lds + BOFF + (wc * NB * 16 + r) * 128;
+        const int c0 = (q ^ (r >> 1)) * 16;         // chunk q of half 0; half 1: chunk q + 4
+        auto read = [&](uint32_t stage, int p) {    // phase p: half p / NP of K, rows p % NP
+            const int kk = p / NP, h = p % NP, c = kk ? c0 ^ 64 : c0;
 #pragma unroll
             for (int m = 0; m < MH; ++m)
-                fa[p & 1][m] = frag(buf, 0, ((h * MH + m) * 2 + wr) * 16 + r, kk);
+                if (h * MH + m < MB)
+                    fa[p & 1][m] = *reinterpret_cast<const u32x4*>(ra + stage + c + (h * MH + m) * WR * 2048);
             if (h == 0)
 #pragma unroll
-                for (int n = 0; n < 4; ++n) fb[kk][n] = frag(buf, 1, wc * 64 + n * 16 + r, kk);
+                for (int n = 0; n < NB; ++n)
+                    fb[kk][n] = *reinterpret_cast<const u32x4*>(rb + stage + c + n * 2048);
         };
 
-        fetch(0);
-        if (steps > 1) {
-            fetch(1);
-            asm volatile("s_waitcnt vmcnt(%0)" :: "n"(CA + 4) : "memory");
-        } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
+        if (steps >= D - 1) asm volatile("s_waitcnt vmcnt(%0)" :: "n"((D - 2) * CA) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         asm volatile("s_barrier" ::: "memory");
         read(0, 0);
+        if (D - 1 < steps) fetch(D - 1, (D - 1) * STAGE);
+        uint32_t cur = 0;
         for (int s = 0; s < steps; ++s) {
-            const int buf = s & 1;
 #pragma unroll
             for (int p = 0; p < PH; ++p) {
                 if (p + 1 < PH) {
-                    read(buf, p + 1);
+                    read(cur, p + 1);
                 } else if (s + 1 < steps) {
-                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n s_barrier" ::: "memory");
-                    read(buf ^ 1, 0);
-                    if (s + 2 < steps) fetch(s + 2);
+                    // Step s + 1 has arrived, and this wave's reads of step s. What may be on its way then:
+                    // D - 2 steps; before step D - 2, whose x was asked for after all the first W, less.
+                    if (s + D - 1 >= steps)
+                        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n s_barrier" ::: "memory");
+                    else if (s < D - 3)
+                        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n s_barrier" :: "n"((D - 2) * CA + CB) : "memory");
+                    else
+                        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n s_barrier" :: "n"((D - 2) * (CA + CB)) : "memory");
+                    const uint32_t free = cur;
+                    cur = cur + STAGE == D * STAGE ? 0 : cur + STAGE;
+                    read(cur, 0);
+                    if (s + D < steps) fetch(s + D, free);
                 }
                 const int kk = p / NP, h = p % NP;
 #pragma unroll
                 for (int m = 0; m < MH; ++m)
+                    if (h * MH + m < MB)
 #pragma unroll
-                    for (int n = 0; n < 4; ++n)
-                        acc[h * MH + m][n] = T::mma(fb[kk][n], fa[p & 1][m], acc[h * MH + m][n]);
+                        for (int n = 0; n < NB; ++n)
+                            acc[h * MH + m][n] = T::mma(fb[kk][n], fa[p & 1][m], acc[h * MH + m][n]);
             }
         }
 
         // A lane holds four neighbouring outputs of row `lane % 16` of each block.
 #pragma unroll
         for (int m = 0; m < MB; ++m) {
-            const int j = (m * 2 + wr) * 16 + r;
+            const int j = (m * WR + wr) * 16 + r;
             if (j >= nr) continue;
             const int id = a.row_ids ? a.row_ids[r0 + j] : 0;
             const bool ok = !a.row_ids || (id >= 0 && id < a.x_rows);
+            constexpr int NF = DUAL ? NB / 2 : NB;
 #pragma unroll
-            for (int n = 0; n < (DUAL ? 2 : 4); ++n) {
+            for (int n = 0; n < NF; ++n) {
                 f32x4 v = acc[m][n];
                 if constexpr (DUAL) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) v[c] = silu_fast(v[c]) * acc[m][n + 2][c];
+                    for (int c = 0; c < 4; ++c) v[c] = silu_fast(v[c]) * acc[m][n + NF][c];
                 }
                 if (!ok) v = (f32x4){0.f, 0.f, 0.f, 0.f};
-                const int f = f0 + wc * (DUAL ? 32 : 64) + 16 * n + 4 * q;
+                const int f = f0 + (wc * NF + n) * 16 + 4 * q;
                 if (f < a.N)
                     store4<T, F32>(a.y, (long)(r0 + j) * a.ldy + f, v, a.N - f, a.vec && f + 4 <= a.N);
             }
@@ -355,46 +436,69 @@ struct TileRun {
     }
 };
 
-template <class T, bool DUAL, bool AL, bool F32>
-__global__ __launch_bounds__(64 * kTileWaves, 2) void grp_tile_kernel(GroupedArgs a) {
-    __shared__ __align__(16) char lds[kTileLds];
-    TileRun<T, DUAL, AL, F32> t{a, lds, 0, 0, 0, 0, (int)(threadIdx.x & 63),
-                                __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)};
+// Up to 256 rows x 256 rows of W, one workgroup of 8 waves to a CU.
+template <class T, bool DUAL, bool F32>
+__global__ __launch_bounds__(512, 2) void grp_tile_kernel(GroupedArgs a) {
+    __shared__ __align__(16) char lds[160 * 1024];
+    TileRun<T, DUAL, F32, 2, 4, 4, 160 * 1024> t{a, lds, 0, 0, 0, 0, (int)(threadIdx.x & 63),
+                                                 __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)};
     if (!find_item(a, 8, t.e, t.r0, t.nr, t.col)) return;
-    if (t.nr <= 64) t.template run<2>();
+    if (t.nr <= 32) t.template run<1>();
+    else if (t.nr <= 64) t.template run<2>();
     else if (t.nr <= 128) t.template run<4>();
+    else if (t.nr <= 160) t.template run<5>();
     else t.template run<8>();
 }
 
-int grouped_tile_rows(long rows, int E) {
-    const long groups = E < rows ? E : rows;
-    const long mean = (rows + groups - 1) / groups;
-    return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 48 ? 64 : 256;
+// Up to 64 rows x 128 rows of W, two workgroups of 4 waves to a CU.
+template <class T, bool DUAL, bool F32>
+__global__ __launch_bounds__(256, 2) void grp_slim_kernel(GroupedArgs a) {
+    __shared__ __align__(16) char lds[80 * 1024];
+    TileRun<T, DUAL, F32, 1, 4, 2, 80 * 1024> t{a, lds, 0, 0, 0, 0, (int)(threadIdx.x & 63),
+                                                __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)};
+    if (!find_item(a, 6, t.e, t.r0, t.nr, t.col)) return;
+    if (t.nr <= 16) t.template run<1>();
+    else if (t.nr <= 32) t.template run<2>();
+    else t.template run<4>();
 }
 
-template <class T, bool DUAL, bool AL, bool F32>
+// Rows per expert up to which the slim kernel runs: gate and up, 6144 -> 2048, 256 experts, at 16 / 32 / 64
+// rows each 2.08 / 2.10 / 3.06 ms against the large kernel's 2.06 / 2.10 / 2.16; at 2 rows 1.83 and
+// 1.95, with 256 features of the 32-row groups of a skewed router 0.294 and 0.361.
+constexpr int kSlimRows = 40;
+
+// Rows per expert, on average over the experts that can have any.
+static long mean_rows(const GroupedArgs& a) {
+    const long rows = (long)a.rows + a.sh_rows, groups = a.E + (a.sh_rows > 0), g = groups < rows ? groups : rows;
+    return (rows + g - 1) / g;
+}
+
+template <class T, bool DUAL, bool F32>
+static int run_tiles(const GroupedArgs& a0, hipStream_t s) {
+    GroupedArgs a = a0;
+    const bool slim = mean_rows(a) <= kSlimRows;
+    const int w = (slim ? 128 : 256) / (DUAL ? 2 : 1);
+    a.ntn = (a.N + w - 1) / w;
+    const long grid = grid_items(a, slim ? 64 : 256);
+    if (grid >= (1L << 31)) return -2;
+    if (slim) hipLaunchKernelGGL((grp_slim_kernel<T, DUAL, F32>), dim3((unsigned)grid), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((grp_tile_kernel<T, DUAL, F32>), dim3((unsigned)grid), dim3(512), 0, s, a);
+    return hipGetLastError() == hipSuccess ? 0 : -4;
+}
+
+template <class T, bool DUAL, bool F32>
 static int run_stream(const GroupedArgs& a0, hipStream_t s) {
     GroupedArgs a = a0;
-    int tb = a.off ? grouped_tile_rows(a.rows, a.E) / 16 : a.tb;
-    if (AL && tb == 16) {
-        const int w = DUAL ? kTileN / 2 : kTileN;
-        a.ntn = (a.N + w - 1) / w;
-        const long items = (a.off ? (long)a.rows / 256 + (a.E < a.rows ? a.E : a.rows) : a.max_tiles) * a.ntn;
-        if (items >= (1L << 31)) return -2;
-        hipLaunchKernelGGL((grp_tile_kernel<T, DUAL, AL, F32>), dim3((unsigned)items),
-                           dim3(64 * kTileWaves), 0, s, a);
-        return hipGetLastError() == hipSuccess ? 0 : -4;
-    }
-    if (tb > 4) tb = 4;
+    const long mean = mean_rows(a);
+    const int tb = mean <= 16 ? 1 : mean <= 32 ? 2 : 4;
     constexpr int NB = DUAL ? 1 : 2;
     a.ntn = (a.N + 16 * NB - 1) / (16 * NB);
-    const long tiles = a.off ? (long)a.rows / (16 * tb) + (a.E < a.rows ? a.E : a.rows) : a.max_tiles;
-    const long grid = tiles * a.ntn;
+    const long grid = grid_items(a, 16 * tb);
     if (grid >= (1L << 31)) return -2;
     const dim3 g((unsigned)grid), b(64 * kStreamWaves);
-    if (tb == 1) hipLaunchKernelGGL((grp_stream_kernel<T, DUAL, NB, 1, 4, AL, F32>), g, b, 0, s, a);
-    else if (tb == 2) hipLaunchKernelGGL((grp_stream_kernel<T, DUAL, NB, 2, 4, AL, F32>), g, b, 0, s, a);
-    else hipLaunchKernelGGL((grp_stream_kernel<T, DUAL, NB, 4, 2, AL, F32>), g, b, 0, s, a);
+    if (tb == 1) hipLaunchKernelGGL((grp_stream_kernel<T, DUAL, NB, 1, 4, false, F32>), g, b, 0, s, a);
+    else if (tb == 2) hipLaunchKernelGGL((grp_stream_kernel<T, DUAL, NB, 2, 4, false, F32>), g, b, 0, s, a);
+    else hipLaunchKernelGGL((grp_stream_kernel<T, DUAL, NB, 4, 2, false, F32>), g, b, 0, s, a);
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }
 
@@ -447,8 +551,8 @@ static int run_types(const GroupedArgs& a, bool f32, hipStream_t s) {
     auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     const bool aligned = a.K % 8 == 0 && a.ldx % 8 == 0 && a.w_stride % 8 == 0 && al(a.x) &&
                          al(a.w0) && (!DUAL || al(a.w1)) && al(a.s0) && al(a.s1);
-    if (aligned) return f32 ? run_stream<T, DUAL, true, true>(a, s) : run_stream<T, DUAL, true, false>(a, s);
-    return f32 ? run_stream<T, DUAL, false, true>(a, s) : run_stream<T, DUAL, false, false>(a, s);
+    if (aligned) return f32 ? run_tiles<T, DUAL, true>(a, s) : run_tiles<T, DUAL, false>(a, s);
+    return f32 ? run_stream<T, DUAL, true>(a, s) : run_stream<T, DUAL, false>(a, s);
 }
 
 int launch_grouped(const GroupedArgs& a0, int dtype, bool f32, hipStream_t s) {

@@ -13,18 +13,15 @@ struct GroupedArgs {
     const int* row_ids;       // [rows] row of x, or null: row r
     const uint16_t *w0, *w1;  // [E] x [N, K], w_stride apart; w1: the up matrices, or null
     long w_stride;
-    const int* off;           // [E + 1], or null: the tile list
-    const int *tiles, *ntiles;// a dispatch's tiles {expert, row, rows, -} of 16 tb rows
-    const uint16_t *s0, *s1;  // tile list: the matrices of expert E (the shared one)
-    int max_tiles, tb;        // tile list: its longest, 16-row blocks per tile
-    int E, rows, N, K;
-    void* y;                  // [rows, N], ldy apart
+    const int* off;           // [E + 1]
+    const uint16_t *s0, *s1;  // sh_rows > 0: the matrices of group E (the shared expert)
+    int sh_row, sh_rows;      // and its rows, after the others'
+    int E, rows, N, K;        // rows: those off counts
+    void* y;                  // a row for each, ldy apart
     long ldy;
     int ntn;                  // set by the launch: workgroups along N, whole-vector stores
     bool vec;
 };
-// Rows per tile the products take for a batch of `rows` rows over E experts.
-int grouped_tile_rows(long rows, int E);
 // dtype: kBf16 or kF16 (x and W); f32: y is fp32, else of that type.
 int launch_grouped(const GroupedArgs& a, int dtype, bool f32, hipStream_t s);
 
