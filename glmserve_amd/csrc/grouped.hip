@@ -96,23 +96,40 @@ __device__ __forceinline__ long xcd_item(long id, long total) {
 // tiles of all experts come before the small ones, each class spread evenly over the XCDs: 16384
 // rows of 16 experts (four large tiles each, half of them with a few rows more) take two rounds of
 // large items and a short one instead of three, 485 -> 410 us.
+// halves: where the small items are at most kFewItems, which leaves half the CUs idle, they come in
+// two halves of the columns, col counting halves (the same case 410 -> 387 us); 1 then, 0 for whole
+// items.
+constexpr int kFewItems = 128;
 __device__ __forceinline__ bool find_item(const GroupedArgs& a, int lg, int& e, int& r0, int& nr,
-                                          int& col) {
+                                          int& col, int* halves = nullptr) {
     const TileScan scan(a, lg);
     long id = blockIdx.x;
     const long big = (long)__builtin_amdgcn_readlane(scan.ibig, 63) * a.ntn;
+    const long small = (long)__builtin_amdgcn_readlane(scan.ismall, 63) * a.ntn;
     const bool large = id < (big + 7) / 8 * 8;
     if (!large) id -= (big + 7) / 8 * 8;
-    const long item = xcd_item(id, large ? big : (long)__builtin_amdgcn_readlane(scan.ismall, 63) * a.ntn);
+    const int split = halves && !large && small <= kFewItems ? 1 : 0;
+    if (halves) *halves = split;
+    const long item = xcd_item(id, large ? big : small << split);
     if (item < 0) return false;
-    col = (int)(item % a.ntn);
-    return scan.find(large, (int)(item / a.ntn), e, r0, nr);
+    const int ntn = a.ntn << split;
+    long t = item / ntn;
+    col = (int)(item % ntn);
+    if (large && a.fours) {
+        // Four tiles at a time: the 32 workgroups that an XCD runs together are 4 x 8 items and read
+        // 12 operands' rows, not 33 (8192^3: 900 -> 854 us).
+        const long nb = big / a.ntn, first = t / 4 * 4, rows = min(4L, nb - first);
+        const long i = item - first * ntn;
+        t = first + i % rows;
+        col = (int)(i / rows);
+    }
+    return scan.find(large, (int)t, e, r0, nr);
 }
 // Workgroups for tiles of `rows` rows: as many as there may be tiles, and what the classes'
-// rounding to 8 adds.
+// rounding to 8 and the halves add.
 static long grid_items(const GroupedArgs& a, int tile_rows) {
     const long groups = a.E + (a.sh_rows > 0), rows = (long)a.rows + a.sh_rows;
-    return (rows / tile_rows + (groups < rows ? groups : rows)) * a.ntn + 16;
+    return (rows / tile_rows + (groups < rows ? groups : rows)) * a.ntn + 16 + kFewItems;
 }
 
 // Few rows per expert: the weights are streamed once and bound the time.
@@ -442,8 +459,14 @@ __global__ __launch_bounds__(512, 2) void grp_tile_kernel(GroupedArgs a) {
     __shared__ __align__(16) char lds[160 * 1024];
     TileRun<T, DUAL, F32, 2, 4, 4, 160 * 1024> t{a, lds, 0, 0, 0, 0, (int)(threadIdx.x & 63),
                                                  __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)};
-    if (!find_item(a, 8, t.e, t.r0, t.nr, t.col)) return;
-    if (t.nr <= 32) t.template run<1>();
+    int halves;
+    if (!find_item(a, 8, t.e, t.r0, t.nr, t.col, &halves)) return;
+    if (halves) {
+        TileRun<T, DUAL, F32, 2, 4, 2, 160 * 1024> h{a, lds, t.e, t.r0, t.nr, t.col, t.lane, t.wv};
+        if (t.nr <= 32) h.template run<1>();
+        else if (t.nr <= 64) h.template run<2>();
+        else h.template run<4>();
+    } else if (t.nr <= 32) t.template run<1>();
     else if (t.nr <= 64) t.template run<2>();
     else if (t.nr <= 128) t.template run<4>();
     else if (t.nr <= 160) t.template run<5>();
@@ -479,6 +502,7 @@ static int run_tiles(const GroupedArgs& a0, hipStream_t s) {
     const bool slim = mean_rows(a) <= kSlimRows;
     const int w = (slim ? 128 : 256) / (DUAL ? 2 : 1);
     a.ntn = (a.N + w - 1) / w;
+    a.fours = mean_rows(a) > 256;                // fewer: an expert's W belongs to one tile
     const long grid = grid_items(a, slim ? 64 : 256);
     if (grid >= (1L << 31)) return -2;
     if (slim) hipLaunchKernelGGL((grp_slim_kernel<T, DUAL, F32>), dim3((unsigned)grid), dim3(256), 0, s, a);

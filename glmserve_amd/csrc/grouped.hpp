@@ -19,8 +19,8 @@ struct GroupedArgs {
     int E, rows, N, K;        // rows: those off counts
     void* y;                  // a row for each, ldy apart
     long ldy;
-    int ntn;                  // set by the launch: workgroups along N, whole-vector stores
-    bool vec;
+    int ntn;                  // set by the launch: workgroups along N, large tiles in fours,
+    bool fours, vec;          // whole-vector stores
 };
 // dtype: kBf16 or kF16 (x and W); f32: y is fp32, else of that type.
 int launch_grouped(const GroupedArgs& a, int dtype, bool f32, hipStream_t s);
