@@ -267,7 +267,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void grp_stream_kernel(GroupedAr
         for (int c = 0; c < TB; ++c) good = c == t ? ok[c] : good;
         if (!good) v = (f32x4){0.f, 0.f, 0.f, 0.f};
         if (j < nr && n < a.N)
-            store4<T, F32>(a.y, (long)(r0 + j) * a.ldy + n, v, a.N - n, a.vec && n + 4 <= a.N);
+            store4<T, F32>(a.y, (long)(r0 + j) * a.ldy + n, v, a.N - n);
     }
 }
 
@@ -283,15 +283,6 @@ __global__ __launch_bounds__(64 * kStreamWaves) void grp_stream_kernel(GroupedAr
 // barrier of a step stands before its last phase: behind it the next step is complete and this
 // step's LDS is free for the step D later.
 constexpr int kTileK = 64;
-__device__ const u32x4 grp_zero = {0u, 0u, 0u, 0u};
-
-// 64 lanes x 16 B from memory to LDS at base + 16 * lane, without the compiler's knowledge: it
-// would have every LDS read wait for all of them.
-__device__ __forceinline__ void copy16(const void* g, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n s_nop 0\n global_load_lds_dwordx4 %0, off"
-                 :: "v"(g), "s"(lds) : "memory");
-}
-
 template <class T, bool DUAL, bool F32, int WR, int WC, int NB, int LDS>
 struct TileRun {
     static constexpr int W = WR * WC, TN = WC * NB * 16;
@@ -323,7 +314,7 @@ struct TileRun {
             const bool whole = k + kTileK <= K;
 #pragma unroll
             for (int i = 0; i < CB; ++i)
-                copy16(whole || k + kb[i] < K ? static_cast<const void*>(pb[i] + k) : &grp_zero,
+                copy16(whole || k + kb[i] < K ? static_cast<const void*>(pb[i] + k) : &kZero16,
                        la + stage + BOFF + (W * i + wv) * 1024);
         };
         auto fetch_x = [&](int s, uint32_t stage) {
@@ -331,7 +322,7 @@ struct TileRun {
             const bool whole = k + kTileK <= K;
 #pragma unroll
             for (int i = 0; i < CA; ++i)
-                copy16(whole || k + ka[i] < K ? static_cast<const void*>(pa[i] + k) : &grp_zero,
+                copy16(whole || k + ka[i] < K ? static_cast<const void*>(pa[i] + k) : &kZero16,
                        la + stage + at[i] * 1024);
         };
         // The first steps' W is on its way while the rows of x are looked up.
@@ -447,7 +438,7 @@ struct TileRun {
                 if (!ok) v = (f32x4){0.f, 0.f, 0.f, 0.f};
                 const int f = f0 + (wc * NF + n) * 16 + 4 * q;
                 if (f < a.N)
-                    store4<T, F32>(a.y, (long)(r0 + j) * a.ldy + f, v, a.N - f, a.vec && f + 4 <= a.N);
+                    store4<T, F32>(a.y, (long)(r0 + j) * a.ldy + f, v, a.N - f);
             }
         }
     }
@@ -579,10 +570,7 @@ static int run_types(const GroupedArgs& a, bool f32, hipStream_t s) {
     return f32 ? run_stream<T, DUAL, true>(a, s) : run_stream<T, DUAL, false>(a, s);
 }
 
-int launch_grouped(const GroupedArgs& a0, int dtype, bool f32, hipStream_t s) {
-    GroupedArgs a = a0;
-    const uintptr_t ya = reinterpret_cast<uintptr_t>(a.y);
-    a.vec = a.ldy % 4 == 0 && ya % (f32 ? 16 : 8) == 0;
+int launch_grouped(const GroupedArgs& a, int dtype, bool f32, hipStream_t s) {
     if (dtype == kBf16) return a.w1 ? run_types<Bf16, true>(a, f32, s) : run_types<Bf16, false>(a, f32, s);
     return a.w1 ? run_types<F16, true>(a, f32, s) : run_types<F16, false>(a, f32, s);
 }

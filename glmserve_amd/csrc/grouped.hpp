@@ -19,8 +19,8 @@ struct GroupedArgs {
     int E, rows, N, K;        // rows: those off counts
     void* y;                  // a row for each, ldy apart
     long ldy;
-    int ntn;                  // set by the launch: workgroups along N, large tiles in fours,
-    bool fours, vec;          // whole-vector stores
+    int ntn;                  // set by the launch: workgroups along N, large tiles in fours
+    bool fours;
 };
 // dtype: kBf16 or kF16 (x and W); f32: y is fp32, else of that type.
 int launch_grouped(const GroupedArgs& a, int dtype, bool f32, hipStream_t s);
@@ -43,8 +43,7 @@ struct LoraArgs {
     long ldy;
     float* part;              // lora_part_bytes: [splits][n][rp], A x of each K split
     int splits, kstep, rp;    // set by the launch: K per split, row length of part,
-    int jn, nx;               // workgroups per token block (by adapter), along N,
-    bool vec;                 // whole-vector loads and stores of base and y
+    int jn, nx;               // workgroups per token block (by adapter), along N
 };
 size_t lora_part_bytes(int n, int L, int K, int r);
 int launch_lora(const LoraArgs& a, int xdt, int wdt, int ydt, hipStream_t s);

@@ -92,7 +92,12 @@ struct XHalf {          // x of the adapters' type
     static __device__ __forceinline__ frag load(const row_t* p, int k) { return load8<AL>(p, k); }
     template <bool AL>
     static __device__ __forceinline__ frag tail(const row_t* p, int k, int K) { return load8_tail<AL>(p, k, K); }
-    static __device__ __forceinline__ f32x4 mma(u32x4 w, const frag& x, f32x4 c) { return W::mma(w, x, c); }
+    // Values 8 c .. 8 c + 7 of a step's row r at p.
+    static __device__ __forceinline__ void lds(const char* p, int c, int r, frag& x) {
+        x = *reinterpret_cast<const u32x4*>(p + (c ^ r) * 16);
+    }
+    static __device__ __forceinline__ u32x4 split(const frag& x) { return x; }
+    static __device__ __forceinline__ f32x4 mma(u32x4 w, u32x4 x, f32x4 c) { return W::mma(w, x, c); }
 };
 template <class W>
 struct XFloat {         // x fp32
@@ -108,8 +113,9 @@ struct XFloat {         // x fp32
 #pragma unroll
             for (int i = 0; i < 4; ++i) { f.v[i] = a[i]; f.v[4 + i] = b[i]; }
         } else {
+            const f32x4 a = *reinterpret_cast<const f32x4_any*>(p + k), b = *reinterpret_cast<const f32x4_any*>(p + k + 4);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f.v[i] = p[k + i];
+            for (int i = 0; i < 4; ++i) { f.v[i] = a[i]; f.v[4 + i] = b[i]; }
         }
         return f;
     }
@@ -120,23 +126,36 @@ struct XFloat {         // x fp32
         for (int i = 0; i < 8; ++i) f.v[i] = k + i < K ? p[k + i] : 0.0f;
         return f;
     }
-    static __device__ __forceinline__ f32x4 mma(u32x4 w, const frag& x, f32x4 c) {
-        return mma3<W>(w, split3(x.v), c);
+    static __device__ __forceinline__ void lds(const char* p, int c, int r, frag& x) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(p + ((2 * c + h) ^ r) * 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.v[4 * h + i] = v[i];
+        }
     }
+    static __device__ __forceinline__ Terms3 split(const frag& x) { return split3(x.v); }
+    static __device__ __forceinline__ f32x4 mma(u32x4 w, const Terms3& x, f32x4 c) { return mma3<W>(w, x, c); }
 };
 
-// The adapters of a block of tokens, one after the other: f(adapter, tokens as a mask of
-// lanes) for every jn-th from j on. id: lane i's token's adapter, -1 for none.
-template <class F>
-__device__ __forceinline__ void each_adapter(int id, int j, int jn, F&& f) {
-    uint64_t rest = __ballot(id >= 0);
-    for (int i = 0; rest; ++i) {
-        const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(rest));
-        const uint64_t m = __ballot(id == a);
-        rest &= ~m;
-        if (i % jn == j) f(a, m);
+// The adapters of a block of tokens, one after the other, every jn-th from the j-th on.
+struct Adapters {
+    int id;                   // lane i: its token's adapter, -1 for none
+    int i;
+    uint64_t rest;
+    __device__ __forceinline__ Adapters(int id_, int j) : id(id_), i(-j), rest(__ballot(id_ >= 0)) {}
+    // The next one and its tokens as a mask of lanes; false after the last.
+    __device__ __forceinline__ bool next(int jn, int& ad, uint64_t& m) {
+        while (rest) {
+            ad = __builtin_amdgcn_readlane(id, __builtin_ctzll(rest));
+            m = __ballot(id == ad);
+            rest &= ~m;
+            const int k = i++;
+            if (k >= 0 && k % jn == 0) return true;
+        }
+        return false;
     }
-}
+};
 __device__ __forceinline__ int block_id(const LoraArgs& a, int t0, int tokens) {
     const int lane = threadIdx.x & 63, t = t0 + lane;
     const int id = lane < tokens && t < a.n ? a.ids[t] : -1;
@@ -146,216 +165,432 @@ __device__ __forceinline__ int rank_of(const LoraArgs& a, int ad) {
     return a.ranks ? min(max(a.ranks[ad], 0), a.r) : a.r;
 }
 
-// part[split][t][:] = A[ids[t]][:, K of the split] x[t][K of the split]. A workgroup:
-// 16 TB tokens, 64 ranks, one split; its waves take chunks of 32 KS of K in turn.
-// A is the MFMA's A operand (D row = rank), x its B (D column = token).
-template <class W, class X, int RB, int TB, bool AL>
-__global__ __launch_bounds__(64 * kLoraWaves) void lora_down_kernel(LoraArgs a) {
-    constexpr int KS = 2, KC = 32 * KS;
-    __shared__ f32x4 red[kLoraWaves][RB * TB][64];
+// part[split][t][:] = A[ids[t]][:, K of the split] x[t][K of the split]. A workgroup: 16 TB
+// tokens, 16 RB ranks, one split, every jn-th adapter of the block: the workgroups of the last j, few
+// of which find an adapter, come first, so that the others fill all XCDs (id % 8) evenly. A is the
+// MFMA's A operand (D row = rank), x its B (D column = token).
+struct DownItem {
+    int split, rank0, j, t0, kb, ke;
+    template <int RB, int TB>
+    static __device__ __forceinline__ DownItem of(const LoraArgs& a) {
+        DownItem d;
+        int id = blockIdx.x;
+        d.split = id % a.splits;
+        id /= a.splits;
+        const int rg = a.rp / 16 > RB ? (a.rp / 16 + RB - 1) / RB : 1;
+        d.rank0 = id % rg * RB * 16;
+        id /= rg;
+        const int blocks = (a.n + 16 * TB - 1) / (16 * TB);
+        d.j = a.jn - 1 - id / blocks;
+        d.t0 = (blocks - 1 - id % blocks) * 16 * TB;
+        d.kb = d.split * a.kstep;
+        d.ke = min(a.K, d.kb + a.kstep);
+        return d;
+    }
+};
+
+// Adds the waves' sums in order and stores those of the tokens in m, ranks from rk on as zeros.
+template <int RB, int TB>
+__device__ __forceinline__ void down_store(const LoraArgs& a, const DownItem& d, const f32x4 (&acc)[RB][TB],
+                                           f32x4 (*red)[RB * TB][64], int rk, uint64_t m) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-    int id = blockIdx.x;
-    const int split = id % a.splits;
-    id /= a.splits;
-    const int rg = a.rp / 16 > RB ? (a.rp / 16 + RB - 1) / RB : 1;
-    const int rank0 = id % rg * RB * 16;
-    id /= rg;
-    const int j = id % a.jn, t0 = id / a.jn * 16 * TB;
-    const int kb = split * a.kstep, ke = min(a.K, kb + a.kstep);
+    __syncthreads();       // what red held before has been read
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int t = 0; t < TB; ++t) red[wv][b * TB + t][lane] = acc[b][t];
+    __syncthreads();
+    for (int f = wv; f < RB * TB; f += kLoraWaves) {
+        const int b = f / TB, t = f % TB, row = d.rank0 + 16 * b + 4 * q, tok = d.t0 + 16 * t + r;
+        f32x4 v = red[0][f][lane];
+#pragma unroll
+        for (int w = 1; w < kLoraWaves; ++w) v += red[w][f][lane];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = row + c < rk ? v[c] : 0.0f;
+        if (row < a.rp && (m >> (16 * t + r) & 1))
+            *reinterpret_cast<f32x4*>(a.part + ((long)d.split * a.n + tok) * a.rp + row) = v;
+    }
+}
+
+// Rows at any address: the waves take chunks of 64 of K in turn, straight to registers.
+template <class W, class X, int RB, int TB>
+__global__ __launch_bounds__(64 * kLoraWaves, 2) void lora_down_kernel(LoraArgs a) {
+    constexpr int KS = 2, KC = 32 * KS;
+    constexpr bool AL = false;
+    __shared__ f32x4 red[kLoraWaves][RB * TB][64];
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const DownItem d = DownItem::of<RB, TB>(a);
+    const int rank0 = d.rank0, t0 = d.t0, j = d.j, kb = d.kb, ke = d.ke;
     const typename X::row_t* xp[TB];
 #pragma unroll
     for (int t = 0; t < TB; ++t) {
         const int tok = t0 + 16 * t + r;
         xp[t] = static_cast<const typename X::row_t*>(a.x) + (long)(tok < a.n ? tok : t0) * a.ldx;
     }
-    each_adapter(block_id(a, t0, 16 * TB), j, a.jn, [&](int ad, uint64_t m) {
+    Adapters list(block_id(a, t0, 16 * TB), j);
+    int ad;
+    uint64_t m;
+    while (list.next(a.jn, ad, m)) {
         const int rk = rank_of(a, ad);
-        const int live = min((rk - rank0 + 15) / 16, RB);     // rank blocks with a rank in use
         f32x4 acc[RB][TB];
         const uint16_t* wp[RB];
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
+            // Rows past the adapter's ranks repeat its last one and are dropped.
             wp[b] = a.A + ((long)ad * a.r + max(min(rank0 + 16 * b + r, rk - 1), 0)) * a.K;
 #pragma unroll
             for (int t = 0; t < TB; ++t) acc[b][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
         }
-        if (live > 0) {
-            int k = kb + wv * KC;
-            for (; k + KC <= ke; k += KC * kLoraWaves) {
+        if (rk > rank0) {
+            struct Chunk {
+                u32x4 w[RB][KS];
+                typename X::frag x[TB][KS];
+            };
+            auto load = [&](Chunk& c, int k) {
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    u32x4 w[RB];
-                    typename X::frag x[TB];
 #pragma unroll
-                    for (int b = 0; b < RB; ++b) w[b] = load8<AL>(wp[b], k + 32 * s + 8 * q);
+                    for (int t = 0; t < TB; ++t) c.x[t][s] = X::template load<AL>(xp[t], k + 32 * s + 8 * q);
 #pragma unroll
-                    for (int t = 0; t < TB; ++t) x[t] = X::template load<AL>(xp[t], k + 32 * s + 8 * q);
+                    for (int b = 0; b < RB; ++b) c.w[b][s] = load8<AL>(wp[b], k + 32 * s + 8 * q);
+                }
+            };
+            auto mul = [&](const Chunk& c) {
 #pragma unroll
-                    for (int b = 0; b < RB; ++b)
+                for (int s = 0; s < KS; ++s)
 #pragma unroll
-                        for (int t = 0; t < TB; ++t) acc[b][t] = X::mma(w[b], x[t], acc[b][t]);
+                    for (int t = 0; t < TB; ++t) {
+                        const auto x = X::split(c.x[t][s]);
+#pragma unroll
+                        for (int b = 0; b < RB; ++b) acc[b][t] = X::mma(c.w[b][s], x, acc[b][t]);
+                    }
+            };
+            constexpr int STEP = KC * kLoraWaves;
+            int k = kb + wv * KC;
+            if (k + KC <= ke) {
+                Chunk c0, c1;
+                load(c0, k);
+                for (;;) {
+                    k += STEP;
+                    const bool more = k + KC <= ke;
+                    if (more) load(c1, k);
+                    mul(c0);
+                    if (!more) break;
+                    k += STEP;
+                    const bool more2 = k + KC <= ke;
+                    if (more2) load(c0, k);
+                    mul(c1);
+                    if (!more2) break;
                 }
             }
             if (k < ke) {
+                Chunk c;
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
                     const int kk = k + 32 * s + 8 * q;
-                    typename X::frag x[TB];
 #pragma unroll
-                    for (int t = 0; t < TB; ++t) x[t] = X::template tail<AL>(xp[t], kk, ke);
+                    for (int t = 0; t < TB; ++t) c.x[t][s] = X::template tail<AL>(xp[t], kk, ke);
 #pragma unroll
-                    for (int b = 0; b < RB; ++b) {
-                        const u32x4 w = load8_tail<AL>(wp[b], kk, ke);
-#pragma unroll
-                        for (int t = 0; t < TB; ++t) acc[b][t] = X::mma(w, x[t], acc[b][t]);
-                    }
+                    for (int b = 0; b < RB; ++b) c.w[b][s] = load8_tail<AL>(wp[b], kk, ke);
                 }
+                mul(c);
             }
         }
-        __syncthreads();       // the last adapter's sums are read
+        down_store<RB, TB>(a, d, acc, red, rk, m);
+    }
+}
+
+// The same for 16-byte aligned rows: steps of 128 of K come to LDS, x and A rows whole (256 or 512 B
+// each), D steps in a ring; wave w has K 32 w .. 32 w + 31 of each step. Chunk c (16 B) of a
+// row is at slot c ^ (row % 16): the 16 rows of a fragment fall on 16 different groups of banks.
+template <class W, class X, int RB, int TB>
+__global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 2 : 1) void lora_down_ring_kernel(LoraArgs a) {
+    constexpr int XB = sizeof(typename X::row_t), XR = 16 * TB, AR = 16 * RB;
+    constexpr int XROW = 128 * XB, XN = XR * XROW / 1024, AN = AR * 256 / 1024;     // instructions of a step
+    constexpr int CX = XN / kLoraWaves, CA = AN / kLoraWaves, C = CX + CA, STEP = (XN + AN) * 1024;
+    constexpr int LDS = (TB == 1 ? 80 : 160) * 1024, D0 = LDS / STEP, D = D0 < 8 ? D0 : 8;
+    static_assert(CX * kLoraWaves == XN && CA * kLoraWaves == AN && D >= 3, "whole instructions");
+    static_assert(kLoraWaves * RB * TB * 1024 <= D * STEP, "the sums take the ring's place");
+    __shared__ __align__(16) char lds[D * STEP];
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const DownItem d = DownItem::of<RB, TB>(a);
+    const int steps = (d.ke - d.kb + 127) / 128;
+    const uint32_t la = lds_addr(lds);
+
+    // This lane's part of a copy: row lane / (chunks of a row) of a piece of 1 KiB, one chunk.
+    constexpr int XL = XROW / 16, AL = 16;
+    const char* px[CX];
+    int kx[CX];                                    // the chunk's first K
+#pragma unroll
+    for (int i = 0; i < CX; ++i) {
+        const int row = (kLoraWaves * i + wv) * (64 / XL) + lane / XL, tok = d.t0 + row;
+        const int c = (lane % XL) ^ (row % 16);
+        kx[i] = d.kb + c * 16 / XB;
+        px[i] = static_cast<const char*>(a.x) + ((long)(tok < a.n ? tok : d.t0) * a.ldx + kx[i]) * XB;
+    }
+    Adapters list(block_id(a, d.t0, XR), d.j);
+    int ad;
+    uint64_t m;
+    while (list.next(a.jn, ad, m)) {
+        const int rk = rank_of(a, ad);
+        f32x4 acc[RB][TB];
 #pragma unroll
         for (int b = 0; b < RB; ++b)
 #pragma unroll
-            for (int t = 0; t < TB; ++t) red[wv][b * TB + t][lane] = acc[b][t];
-        __syncthreads();
-        for (int f = wv; f < RB * TB; f += kLoraWaves) {
-            const int b = f / TB, t = f % TB, row = rank0 + 16 * b + 4 * q, tok = t0 + 16 * t + r;
-            f32x4 v = red[0][f][lane];
+            for (int t = 0; t < TB; ++t) acc[b][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        if (rk > d.rank0) {
+            const uint16_t* pa[CA];
+            int ka[CA];
 #pragma unroll
-            for (int w = 1; w < kLoraWaves; ++w) v += red[w][f][lane];
+            for (int i = 0; i < CA; ++i) {
+                // Rows past the adapter's ranks repeat its last one and are dropped.
+                const int row = (kLoraWaves * i + wv) * 4 + lane / AL;
+                ka[i] = d.kb + ((lane % AL) ^ (row % 16)) * 8;
+                pa[i] = a.A + ((long)ad * a.r + min(d.rank0 + row, rk - 1)) * a.K + ka[i];
+            }
+            auto fetch = [&](int s, uint32_t slot) __attribute__((always_inline)) {
+                const int k = s * 128;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) v[c] = row + c < rk ? v[c] : 0.0f;
-            if (row < a.rp && (m >> (16 * t + r) & 1))
-                *reinterpret_cast<f32x4*>(a.part + ((long)split * a.n + tok) * a.rp + row) = v;
+                for (int i = 0; i < CX; ++i)
+                    copy16(k + kx[i] < d.ke ? static_cast<const void*>(px[i] + k * XB) : &kZero16,
+                           la + slot + (kLoraWaves * i + wv) * 1024);
+#pragma unroll
+                for (int i = 0; i < CA; ++i)
+                    copy16(k + ka[i] < d.ke ? static_cast<const void*>(pa[i] + k) : &kZero16,
+                           la + slot + XN * 1024 + (kLoraWaves * i + wv) * 1024);
+            };
+            __syncthreads();                       // the last adapter's sums are read
+#pragma unroll
+            for (int s = 0; s < D - 1; ++s)
+                if (s < steps) fetch(s, s * STEP);
+            uint32_t cur = 0, fill = (D - 1) * STEP;
+            for (int s = 0; s < steps; ++s) {
+                // Step s has arrived, and every wave has read step s - 1.
+                if (s + D - 2 < steps)
+                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n s_barrier" :: "n"((D - 2) * C) : "memory");
+                else
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n s_barrier" ::: "memory");
+                u32x4 w[RB];
+                typename X::frag x[TB];
+                const char* xs = lds + cur + r * XROW;
+#pragma unroll
+                for (int t = 0; t < TB; ++t) X::lds(xs + t * 16 * XROW, 4 * wv + q, r, x[t]);
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+                    w[b] = *reinterpret_cast<const u32x4*>(lds + cur + XN * 1024 + (16 * b + r) * 256 +
+                                                           ((4 * wv + q) ^ r) * 16);
+                if (s + D - 1 < steps) fetch(s + D - 1, fill);
+                fill = cur;
+                cur = cur + STEP == D * STEP ? 0 : cur + STEP;
+#pragma unroll
+                for (int t = 0; t < TB; ++t) {
+                    const auto xx = X::split(x[t]);
+#pragma unroll
+                    for (int b = 0; b < RB; ++b) acc[b][t] = X::mma(w[b], xx, acc[b][t]);
+                }
+            }
         }
-    });
+        down_store<RB, TB>(a, d, acc, reinterpret_cast<f32x4 (*)[RB * TB][64]>(lds), rk, m);
+    }
 }
 
-// Four values of a row of base / y as fp32.
+// Element type of base and y: fp32 or a 16-bit type.
 template <int DT>
-__device__ __forceinline__ f32x4 get4(const void* p, long at, int cnt, bool vec) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (DT == kF32) {
-        const float* f = static_cast<const float*>(p) + at;
-        if (vec) return *reinterpret_cast<const f32x4*>(f);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < cnt) v[i] = f[i];
-    } else {
-        const uint16_t* h = static_cast<const uint16_t*>(p) + at;
-        u32x2 w = {0u, 0u};
-        if (vec) {
-            w = *reinterpret_cast<const u32x2*>(h);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i < cnt) w[i / 2] |= (uint32_t)h[i] << (16 * (i & 1));
-        }
+struct Out {
+    typedef uint16_t elem;
+    static __device__ __forceinline__ float get(const elem* p) { return DT == kBf16 ? Bf16::up(*p) : F16::up(*p); }
+    static __device__ __forceinline__ void put(elem* p, float v) {
+        *p = (uint16_t)(DT == kBf16 ? Bf16::pack2(v, v) : F16::pack2(v, v));
+    }
+    static __device__ __forceinline__ f32x4 get4(const elem* p) {
+        const u32x2 w = *reinterpret_cast<const u32x2_any*>(p);
+        f32x4 v;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t u = w[i / 2] >> (16 * (i & 1));
             v[i] = DT == kBf16 ? Bf16::up(u) : F16::up(u);
         }
+        return v;
     }
-    return v;
-}
-template <int DT>
-__device__ __forceinline__ void put4(void* p, long at, f32x4 v, int cnt, bool vec) {
-    if constexpr (DT == kF16) store4<F16, false>(p, at, v, cnt, vec);
-    else store4<Bf16, DT == kF32>(p, at, v, cnt, vec);
-}
+    static __device__ __forceinline__ void put4(elem* p, f32x4 v) {
+        if constexpr (DT == kBf16) store4<Bf16, false>(p, 0, v, 4);
+        else store4<F16, false>(p, 0, v, 4);
+    }
+};
+template <>
+struct Out<kF32> {
+    typedef float elem;
+    static __device__ __forceinline__ float get(const float* p) { return *p; }
+    static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+    static __device__ __forceinline__ f32x4 get4(const float* p) { return *reinterpret_cast<const f32x4_any*>(p); }
+    static __device__ __forceinline__ void put4(float* p, f32x4 v) { *reinterpret_cast<f32x4_any*>(p) = v; }
+};
 
 // y = base + scale * B (sum of part over the splits). A workgroup: 16 TB tokens, 256
-// columns, 64 per wave; A x is summed, cut into three bf16 terms and kept in LDS.
-// B is the MFMA's A operand (D row = output), A x its B (D column = token): a lane has
-// four neighbouring outputs of one token.
-template <class W, int YD, int TB, bool AL>
-__global__ __launch_bounds__(64 * kLoraWaves) void lora_up_kernel(LoraArgs a) {
+// columns, 64 per wave; A x is summed, cut into three bf16 terms and kept in LDS, while the first
+// adapter's rows of B and its tokens' base are on their way. B is the MFMA's A operand (D row =
+// output), A x its B (D column = token): a lane has four neighbouring outputs of one token. The up to
+// three columns after N's last four are plain dot products.
+template <class W, int YD, int TB>
+__global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 4 : 2) void lora_up_kernel(LoraArgs a) {
     constexpr int NB = 4;
-    extern __shared__ uint16_t terms[];              // [3][16 TB][stride]
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-    const int stride = (a.r + 31) / 32 * 32 + 8;
+    typedef Out<YD> O;
+    typedef typename O::elem elem;
+    extern __shared__ __align__(16) uint16_t terms[];            // [3][16 TB][stride]
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int r = lane & 15, q = lane >> 4, stride = (a.r + 31) / 32 * 32 + 8;
     int id = blockIdx.x;
     const int n0 = (id % a.nx * kLoraWaves + wv) * 16 * NB;
     id /= a.nx;
-    const int j = id % a.jn, t0 = id / a.jn * 16 * TB;
+    const int blocks = (a.n + 16 * TB - 1) / (16 * TB);
+    const int j = a.jn - 1 - id / blocks, t0 = (blocks - 1 - id % blocks) * 16 * TB;   // as in the first launch
     const int ad0 = block_id(a, t0, 16 * TB);
     const uint64_t has = __ballot(ad0 >= 0);
-    auto word = [&](int term, int t, int k) { return terms + ((term * 16 * TB + t) * stride + k); };
+    Adapters list(ad0, j);
+    int ad;
+    uint64_t m;
+    bool some = list.next(a.jn, ad, m);
+    const int left = min(a.n - t0, 16 * TB);
+    // Tokens without an adapter are copied; in place they are there already.
+    const uint64_t none = j == 0 && a.y != a.base ? ~has & (left >= 64 ? ~0ull : (1ull << left) - 1) : 0;
+    if (!some && !none) return;
 
-    for (int i = threadIdx.x; i < 16 * TB * (stride / 8); i += 64 * kLoraWaves) {
-        const int t = i / (stride / 8), k = i % (stride / 8) * 8;
+    const int n4 = a.N & ~3, nl = n0 + 4 * q;                    // whole fours; the lane's first column
+    const elem* pb = static_cast<const elem*>(a.base) + (long)(t0 + r) * a.ldb + nl;
+    elem* py = static_cast<elem*>(a.y) + (long)(t0 + r) * a.ldy + nl;
+    f32x4 base[TB][NB];
+    u32x4 w[NB];
+    const uint16_t* wp[NB];
+    int rk = 0;
+    auto load_w = [&](int k) __attribute__((always_inline)) {
+        if (rk % 8 == 0) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                w[b] = (u32x4){0u, 0u, 0u, 0u};
+                if (k + 8 * q < rk) w[b] = load8<false>(wp[b], k + 8 * q);
+            }
+        } else {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) w[b] = load8_tail<false>(wp[b], k + 8 * q, rk);
+        }
+    };
+    auto load_base = [&](uint64_t mask) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < TB; ++t)
+            if (mask >> (16 * t + r) & 1) {
+                const elem* p = pb + 16L * t * a.ldb;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    if (nl + 16 * b < n4) base[t][b] = O::get4(p + 16 * b);
+            }
+    };
+    auto begin = [&]() __attribute__((always_inline)) {
+        rk = rank_of(a, ad);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) wp[b] = a.B + ((long)ad * a.N + min(n0 + 16 * b + r, a.N - 1)) * a.r;
+        load_w(0);
+        load_base(m);
+    };
+    if (some) begin();
+
+    const int segs = stride / 8;
+    for (int i = threadIdx.x; i < 16 * TB * segs; i += 64 * kLoraWaves) {
+        const int t = i / segs, k = i % segs * 8;
         float v[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) v[c] = 0.0f;
         if (k < a.rp && (has >> t & 1)) {
-            for (int s = 0; s < a.splits; ++s) {
-                const float* p = a.part + ((long)s * a.n + t0 + t) * a.rp + k;
+            const float* p = a.part + (long)(t0 + t) * a.rp + k;
+            const long step = (long)a.n * a.rp;
+            for (int s = 0; s < a.splits; s += 4) {
+                f32x4 u[4][2];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) v[c] += p[c];
+                for (int d = 0; d < 4; ++d) {
+                    const float* ps = p + min(s + d, a.splits - 1) * step;
+                    u[d][0] = *reinterpret_cast<const f32x4*>(ps);
+                    u[d][1] = *reinterpret_cast<const f32x4*>(ps + 4);
+                }
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) v[c] = s + d < a.splits ? v[c] + u[d][c / 4][c % 4] : v[c];
             }
         }
         const Terms3 o = split3(v);
 #pragma unroll
-        for (int c = 0; c < 3; ++c) *reinterpret_cast<u32x4*>(word(c, t, k)) = o.t[c];
+        for (int c = 0; c < 3; ++c) *reinterpret_cast<u32x4*>(terms + (c * 16 * TB + t) * stride + k) = o.t[c];
     }
     __syncthreads();
 
-    auto each_out = [&](uint64_t m, auto&& value) {
-#pragma unroll
-        for (int t = 0; t < TB; ++t) {
-            const int tok = t0 + 16 * t + r;
-            if (!(m >> (16 * t + r) & 1)) continue;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const int n = n0 + 16 * b + 4 * q;
-                if (n >= a.N) continue;
-                const bool vec = a.vec && n + 4 <= a.N;
-                const f32x4 v = get4<YD>(a.base, (long)tok * a.ldb + n, a.N - n, vec);
-                put4<YD>(a.y, (long)tok * a.ldy + n, value(b, t, v), a.N - n, vec);
-            }
-        }
-    };
-    if (j == 0 && a.y != a.base) {                    // tokens without an adapter
-        const int left = a.n - t0;
-        const uint64_t here = left >= 64 ? ~0ull : (1ull << left) - 1;
-        const uint64_t none = ~has & here & (TB == 4 ? ~0ull : (1ull << (16 * TB)) - 1);
-        each_out(none, [](int, int, f32x4 v) { return v; });
-    }
-    each_adapter(ad0, j, a.jn, [&](int ad, uint64_t m) {
-        const int rk = rank_of(a, ad);
+    const bool last = n4 < a.N && n0 <= n4 && n4 < n0 + 16 * NB;   // this wave has N's last columns
+    while (some) {
         const float sc = a.scale ? a.scale[ad] : 1.0f;
         f32x4 acc[NB][TB];
-        const uint16_t* wp[NB];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            wp[b] = a.B + ((long)ad * a.N + min(n0 + 16 * b + r, a.N - 1)) * a.r;
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int t = 0; t < TB; ++t) acc[b][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        }
         for (int k = 0; k < rk; k += 32) {
-            const int kk = k + 8 * q;
-            Terms3 x[TB];
+            if (k) load_w(k);
 #pragma unroll
-            for (int t = 0; t < TB; ++t)
+            for (int t = 0; t < TB; ++t) {
+                Terms3 x;
 #pragma unroll
-                for (int c = 0; c < 3; ++c) x[t].t[c] = *reinterpret_cast<const u32x4*>(word(c, 16 * t + r, kk));
+                for (int c = 0; c < 3; ++c)
+                    x.t[c] = *reinterpret_cast<const u32x4*>(terms + ((c * TB + t) * 16 + r) * stride + k + 8 * q);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const u32x4 w = load8_tail<false>(wp[b], kk, rk);
-#pragma unroll
-                for (int t = 0; t < TB; ++t) acc[b][t] = mma3<W>(w, x[t], acc[b][t]);
+                for (int b = 0; b < NB; ++b) acc[b][t] = mma3<W>(w[b], x, acc[b][t]);
             }
         }
-        each_out(m, [&](int b, int t, f32x4 v) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) v[c] = __builtin_fmaf(sc, acc[b][t][c], v[c]);
-            return v;
-        });
-    });
+        for (int t = 0; t < TB; ++t)
+            if (m >> (16 * t + r) & 1) {
+                elem* p = py + 16L * t * a.ldy;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    if (nl + 16 * b < n4) {
+                        f32x4 v;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) v[c] = __builtin_fmaf(sc, acc[b][t][c], base[t][b][c]);
+                        O::put4(p + 16 * b, v);
+                    }
+            }
+        if (last && lane < 16 * TB && (m >> lane & 1))
+            for (int n = n4; n < a.N; ++n) {
+                const uint16_t* row = a.B + ((long)ad * a.N + n) * a.r;
+                float v = 0.0f;
+                for (int k = 0; k < rk; ++k) {
+                    const uint16_t* t = terms + lane * stride + k;
+                    const float x = (Bf16::up(t[0]) + Bf16::up(t[16 * TB * stride])) + Bf16::up(t[32 * TB * stride]);
+                    v = __builtin_fmaf(W::up(row[k]), x, v);
+                }
+                const elem* p = static_cast<const elem*>(a.base) + (long)(t0 + lane) * a.ldb + n;
+                O::put(static_cast<elem*>(a.y) + (long)(t0 + lane) * a.ldy + n, __builtin_fmaf(sc, v, O::get(p)));
+            }
+        some = list.next(a.jn, ad, m);
+        if (some) begin();
+    }
+    if (none) {
+        load_base(none);
+#pragma unroll
+        for (int t = 0; t < TB; ++t)
+            if (none >> (16 * t + r) & 1) {
+                elem* p = py + 16L * t * a.ldy;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    if (nl + 16 * b < n4) O::put4(p + 16 * b, base[t][b]);
+            }
+        if (last && lane < 16 * TB && (none >> lane & 1))
+            for (int n = n4; n < a.N; ++n)
+                static_cast<elem*>(a.y)[(long)(t0 + lane) * a.ldy + n] =
+                    static_cast<const elem*>(a.base)[(long)(t0 + lane) * a.ldb + n];
+    }
 }
 
-// How the first launch splits K: enough workgroups to fill the chip, 256 of K at least.
+// How the first launch splits K: 512 workgroups (with 256 / 1024 the case above takes 125 / 110 us), 512 of
+// K at least.
 struct LoraPlan {
     int tb, blocks, jn, splits, kstep, rp;
 };
@@ -364,11 +599,15 @@ static LoraPlan plan_of(int n, int L, int K, int r) {
     p.tb = n > 1024 ? 2 : 1;
     p.blocks = (n + 16 * p.tb - 1) / (16 * p.tb);
     const int most = n < L ? n : L;
-    p.jn = n > 512 ? 1 : most < 16 ? most : 16;
+    // Workgroups per block of tokens, over its adapters: a batch of decoding tokens has up to 16 in a
+    // block, a long one is mostly prompts with one, and a workgroup that finds no adapter costs its
+    // start (4096 tokens of 8 prompts and 32 decoding tokens: 146 / 85 / 87 us with 1 / 2 / 4).
+    const int jn = n <= 1024 ? 16 : n <= 8192 ? 2 : 1;
+    p.jn = most < jn ? most : jn;
     p.rp = (r + 15) / 16 * 16;
-    const long wgs = (long)p.blocks * p.jn * ((r + 16 * kRankBlocks - 1) / (16 * kRankBlocks));
+    const long wgs = (long)p.blocks * (n <= 256 ? p.jn : 1) * ((r + 16 * kRankBlocks - 1) / (16 * kRankBlocks));
     long s = (512 + wgs - 1) / wgs;
-    const int top = (K + 255) / 256;
+    const int top = (K + 511) / 512;
     s = s < 1 ? 1 : s > top ? top : s;
     p.kstep = (int)(((K + s - 1) / s + 127) / 128 * 128);
     p.splits = (K + p.kstep - 1) / p.kstep;
@@ -379,18 +618,22 @@ size_t lora_part_bytes(int n, int L, int K, int r) {
     return (size_t)p.splits * n * p.rp * 4;
 }
 
-template <class W, class X, bool AL>
-static void run_down(const LoraArgs& a, const LoraPlan& p, unsigned grid, hipStream_t s) {
+template <class W, class X>
+static void run_down(const LoraArgs& a, const LoraPlan& p, bool aligned, unsigned grid, hipStream_t s) {
     const dim3 g(grid), b(64 * kLoraWaves);
     const int rb = p.rp / 16;
-    auto go = [&](auto tb) {
-        constexpr int TB = decltype(tb)::value;
-        if (rb == 1) hipLaunchKernelGGL((lora_down_kernel<W, X, 1, TB, AL>), g, b, 0, s, a);
-        else if (rb == 2) hipLaunchKernelGGL((lora_down_kernel<W, X, 2, TB, AL>), g, b, 0, s, a);
-        else hipLaunchKernelGGL((lora_down_kernel<W, X, 4, TB, AL>), g, b, 0, s, a);
+    auto go = [&](auto tb, auto r) {
+        constexpr int TB = decltype(tb)::value, RB = decltype(r)::value;
+        if (aligned) hipLaunchKernelGGL((lora_down_ring_kernel<W, X, RB, TB>), g, b, 0, s, a);
+        else hipLaunchKernelGGL((lora_down_kernel<W, X, RB, TB>), g, b, 0, s, a);
     };
-    if (p.tb == 1) go(std::integral_constant<int, 1>{});
-    else go(std::integral_constant<int, 2>{});
+    auto ranks = [&](auto tb) {
+        if (rb == 1) go(tb, std::integral_constant<int, 1>{});
+        else if (rb == 2) go(tb, std::integral_constant<int, 2>{});
+        else go(tb, std::integral_constant<int, 4>{});
+    };
+    if (p.tb == 1) ranks(std::integral_constant<int, 1>{});
+    else ranks(std::integral_constant<int, 2>{});
 }
 
 template <class W, int YD>
@@ -399,13 +642,12 @@ static int run_up(const LoraArgs& a0, hipStream_t s) {
     const int tb = a.n > 1024 && a.r <= 128 ? 4 : 1;   // 52 KiB of LDS at most
     const long blocks = (a.n + 16 * tb - 1) / (16 * tb);
     a.nx = (a.N + 255) / 256;
-    if (tb == 4) a.jn = 1;
     const long grid = blocks * a.jn * a.nx;
     if (grid >= (1L << 31)) return -2;
     const size_t lds = (size_t)3 * 16 * tb * ((a.r + 31) / 32 * 32 + 8) * 2;
     const dim3 g((unsigned)grid), b(64 * kLoraWaves);
-    if (tb == 1) hipLaunchKernelGGL((lora_up_kernel<W, YD, 1, true>), g, b, lds, s, a);
-    else hipLaunchKernelGGL((lora_up_kernel<W, YD, 4, true>), g, b, lds, s, a);
+    if (tb == 1) hipLaunchKernelGGL((lora_up_kernel<W, YD, 1>), g, b, lds, s, a);
+    else hipLaunchKernelGGL((lora_up_kernel<W, YD, 4>), g, b, lds, s, a);
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }
 
@@ -414,16 +656,14 @@ int launch_lora(const LoraArgs& a0, int xdt, int wdt, int ydt, hipStream_t s) {
     const LoraPlan p = plan_of(a.n, a.L, a.K, a.r);
     a.splits = p.splits, a.kstep = p.kstep, a.rp = p.rp, a.jn = p.jn;
     auto al = [](const void* q, size_t v) { return reinterpret_cast<uintptr_t>(q) % v == 0; };
-    const size_t yb = ydt == kF32 ? 16 : 8;
-    a.vec = a.ldb % 4 == 0 && a.ldy % 4 == 0 && al(a.base, yb) && al(a.y, yb);
     const bool aligned = a.K % 8 == 0 && al(a.x, 16) && al(a.A, 16) && a.ldx % (xdt == kF32 ? 4 : 8) == 0;
     const long grid = (long)p.blocks * p.jn * ((p.rp / 16 + kRankBlocks - 1) / kRankBlocks) * p.splits;
     if (grid >= (1L << 31)) return -2;
     auto down = [&](auto w) {
         using W = decltype(w);
         const unsigned g = (unsigned)grid;
-        if (xdt == kF32) aligned ? run_down<W, XFloat<W>, true>(a, p, g, s) : run_down<W, XFloat<W>, false>(a, p, g, s);
-        else aligned ? run_down<W, XHalf<W>, true>(a, p, g, s) : run_down<W, XHalf<W>, false>(a, p, g, s);
+        if (xdt == kF32) run_down<W, XFloat<W>>(a, p, aligned, g, s);
+        else run_down<W, XHalf<W>>(a, p, aligned, g, s);
     };
     if (wdt == kBf16) down(Bf16{});
     else down(F16{});

@@ -8,7 +8,10 @@ namespace glmmoe {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+// The same vectors at any address of their elements: the memory pipeline takes them there.
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 // Data type codes of the C entries (GLMMOE_F32 / BF16 / F16).
 constexpr int kF32 = 0, kBf16 = 1, kF16 = 2;
@@ -71,26 +74,36 @@ __device__ __forceinline__ u32x4 load8_tail(const uint16_t* row, int k, int K) {
     return v;
 }
 
-// Four consecutive outputs of a row, the first `cnt` of them: one store where VEC.
+// 16 bytes of zeros in memory, for copies of what lies past a row's end.
+static __device__ const u32x4 kZero16 = {0u, 0u, 0u, 0u};
+
+// 64 lanes x 16 B from memory to LDS at base + 16 * lane, without the compiler's knowledge: it
+// would have every LDS read wait for all of them.
+__device__ __forceinline__ void copy16(const void* g, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n s_nop 0\n global_load_lds_dwordx4 %0, off"
+                 :: "v"(g), "s"(lds) : "memory");
+}
+
+// Four consecutive outputs of a row from element `at` on, of which cnt are inside it.
 template <class T, bool F32>
-__device__ __forceinline__ void store4(void* y, long at, f32x4 v, int cnt, bool vec) {
+__device__ __forceinline__ void store4(void* y, long at, f32x4 v, int cnt) {
     if constexpr (F32) {
         float* p = static_cast<float*>(y) + at;
-        if (vec) {
-            *reinterpret_cast<f32x4*>(p) = v;
+        if (cnt >= 4) {
+            *reinterpret_cast<f32x4_any*>(p) = v;
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 3; ++i)
                 if (i < cnt) p[i] = v[i];
         }
     } else {
         uint16_t* p = static_cast<uint16_t*>(y) + at;
         const u32x2 w = {T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
-        if (vec) {
-            *reinterpret_cast<u32x2*>(p) = w;
+        if (cnt >= 4) {
+            *reinterpret_cast<u32x2_any*>(p) = w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 3; ++i)
                 if (i < cnt) p[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
         }
     }
