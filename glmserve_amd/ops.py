@@ -4,7 +4,6 @@ Names, argument order and meaning follow the reference launchers; tensors are
 device tensors and `stream` is a torch.cuda.Stream or None (current stream).
 Unlike the reference (void return, errors printed), failures raise GlmMoeError.
 """
-import contextlib
 import ctypes
 
 import torch
@@ -249,14 +248,23 @@ class BF16MoELayer(_MoELayer):
 # ---- Ragged products on 16-bit weights -------------------------------------------
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_HALF = (torch.bfloat16, torch.float16)
 
 
-_HERE = contextlib.nullcontext()
+def _stream_on(stream, idx):
+    """Raw handle of `stream`, or of the current stream of device idx."""
+    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(idx)
 
 
-def _on(dev):
-    """Makes dev the current device for a call (nothing to do where it is)."""
-    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+def _call(fn, what, idx, args):
+    """fn(*args) with device idx current."""
+    if torch._C._cuda_getDevice() == idx:
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args)
+    if rc:
+        check(rc, what)
 
 
 def _need_rows(t, dtypes, rows, cols, name, device=None):
@@ -283,25 +291,50 @@ def _stack(w, E, N, K, dtype, name, device):
     return w.stride(0) if E > 1 else N * K
 
 
-def _grouped(what, x, ws, expert_offsets, y, row_ids, stream):
+def _refuse_grouped(what, x, ws, expert_offsets, y, row_ids):
+    """Says what is wrong with the arguments of a grouped product."""
     half = (torch.bfloat16, torch.float16)
     if x is None or x.dim() != 2 or ws[0].dim() != 3 or y is None or y.dim() != 2:
         raise GlmMoeError(f"{what}: expected x [rows, K], weights [E, N, K] and an output [rows, N]")
     dev = x.device
     E, N, K = ws[0].shape
     rows = y.shape[0]
-    ldx = _need_rows(x, half, rows if row_ids is None else 0, K, "x")
-    strides = [_stack(w, E, N, K, x.dtype, "w", dev) for w in ws]
-    if len(set(strides)) > 1:
+    _need_rows(x, half, rows if row_ids is None else 0, K, "x")
+    if len({_stack(w, E, N, K, x.dtype, "w", dev) for w in ws}) > 1:
         raise GlmMoeError(f"{what}: the two weight tensors have different expert strides")
-    ldy = _need_rows(y, (torch.float32, x.dtype), 0, N, "y", dev)
+    _need_rows(y, (torch.float32, x.dtype), 0, N, "y", dev)
     _need_on(expert_offsets, torch.int32, E + 1, "expert_offsets", dev)
     if row_ids is not None:
         _need_on(row_ids, torch.int32, rows, "row_ids", dev)
-    with _on(dev):
-        check(getattr(lib(), "glmmoe_" + what)(
-            _DTYPE[x.dtype], _p(x), ldx, x.shape[0], _p(row_ids), *[_p(w) for w in ws], strides[0],
-            _p(expert_offsets), E, rows, N, K, _DTYPE[y.dtype], _p(y), ldy, _s(stream)), what)
+    raise GlmMoeError(f"{what}: unsupported arguments")
+
+
+def _grouped(what, x, w, w2, expert_offsets, y, row_ids, stream):
+    # One pass over what a call may look like; anything else is looked at again, to say why not.
+    try:
+        (E, N, K), (rows, ny), (xr, kx) = w.shape, y.shape, x.shape
+        idx, dt, (ldx, cx), (ldy, cy), sw = x.get_device(), x.dtype, x.stride(), y.stride(), w.stride()
+        ok = (idx >= 0 and kx == K and ny == N and dt in _HALF and w.dtype == dt and y.dtype in (dt, torch.float32)
+              and (cx == 1 or K == 1) and (cy == 1 or N == 1) and (sw[2] == 1 or K == 1) and (sw[1] == K or N == 1)
+              and w.get_device() == idx and y.get_device() == idx and expert_offsets.get_device() == idx
+              and expert_offsets.dtype == torch.int32 and expert_offsets.is_contiguous()
+              and expert_offsets.numel() > E)
+        if row_ids is None:
+            ok = ok and xr >= rows
+        else:
+            ok = (ok and row_ids.get_device() == idx and row_ids.dtype == torch.int32 and row_ids.is_contiguous()
+                  and row_ids.numel() >= rows)
+        if w2 is not None:
+            ok = ok and w2.get_device() == idx and w2.dtype == dt and w2.shape == w.shape and w2.stride() == sw
+    except (AttributeError, TypeError, ValueError):
+        ok = False
+    if not ok:
+        _refuse_grouped(what, x, (w,) if w2 is None else (w, w2), expert_offsets, y, row_ids)
+    weights = (w.data_ptr(),) if w2 is None else (w.data_ptr(), w2.data_ptr())
+    _call(getattr(lib(), "glmmoe_" + what), what, idx,
+          (_DTYPE[dt], x.data_ptr(), ldx if xr > 1 else K, xr, None if row_ids is None else row_ids.data_ptr(),
+           *weights, sw[0] if E > 1 else N * K, expert_offsets.data_ptr(), E, rows, N, K, _DTYPE[y.dtype],
+           y.data_ptr(), ldy if rows > 1 else N, _stream_on(stream, idx)))
 
 
 def grouped_linear(x, w, expert_offsets, y, row_ids=None, stream=None):
@@ -310,17 +343,44 @@ def grouped_linear(x, w, expert_offsets, y, row_ids=None, stream=None):
     x [*, K] and w [E, N, K] bf16 or fp16; y [rows, N] of x's type or fp32; rows of x and y,
     and the matrices of w, may be strided. expert_offsets [E + 1], row_ids [rows] int32.
     Rows outside the offsets are left as they are."""
-    _grouped("grouped_linear", x, (w,), expert_offsets, y, row_ids, stream)
+    _grouped("grouped_linear", x, w, None, expert_offsets, y, row_ids, stream)
 
 
 def grouped_gate_up(x, w_gate, w_up, expert_offsets, h, row_ids=None, stream=None):
     """h[r] = silu(w_gate[e] @ x) * (w_up[e] @ x), x and the rows as grouped_linear takes
     them; w_gate and w_up [E, N, K] may be the halves of one [E, 2 N, K] tensor."""
-    _grouped("grouped_gate_up", x, (w_gate, w_up), expert_offsets, h, row_ids, stream)
+    if w_up is None:
+        raise GlmMoeError("grouped_gate_up: expected w_up")
+    _grouped("grouped_gate_up", x, w_gate, w_up, expert_offsets, h, row_ids, stream)
 
 
 def lora_workspace_bytes(n, n_adapters, K, r):
+    """Bytes of lora_add's workspace for n tokens."""
     return lib().glmmoe_lora_workspace_bytes(n, n_adapters, K, r)
+
+
+def _refuse_lora(x, adapter_ids, A, B, scale, base, y, ranks, ws):
+    """Says what is wrong with lora_add's arguments."""
+    if x.dim() != 2 or A.dim() != 3 or B.dim() != 3 or A.dtype not in _HALF:
+        raise GlmMoeError("lora_add: expected x [n, K], A [adapters, r, K] and B [adapters, N, r], bf16 or fp16")
+    dev = x.device
+    L, r, K = A.shape
+    N, n = B.shape[1], x.shape[0]
+    _need_on(A, A.dtype, L * r * K, "A", dev)
+    if tuple(B.shape) != (L, N, r):
+        raise GlmMoeError(f"B: expected [{L}, {N}, {r}]")
+    _need_on(B, A.dtype, L * N * r, "B", dev)
+    _need_rows(x, (torch.float32, A.dtype), n, K, "x")
+    _need_on(adapter_ids, torch.int32, n, "adapter_ids", dev)
+    _need_rows(base, (torch.float32, A.dtype), n, N, "base", dev)
+    _need_rows(y, (base.dtype,), n, N, "y", dev)
+    if scale is not None:
+        _need_on(scale, torch.float32, L, "scale", dev)
+    if ranks is not None:
+        _need_on(ranks, torch.int32, L, "ranks", dev)
+    if ws is not None:
+        _need_on(ws, torch.uint8, 0, "ws", dev)
+    raise GlmMoeError("lora_add: unsupported arguments")
 
 
 def lora_add(x, adapter_ids, A, B, scale, base, y, ranks=None, ws=None, stream=None):
@@ -330,34 +390,40 @@ def lora_add(x, adapter_ids, A, B, scale, base, y, ranks=None, ws=None, stream=N
     base and y [n, N] fp32 or the adapters' type, the same tensor to add in place. ranks
     [n_adapters] int32: ranks in use of each adapter. ws: a uint8 tensor of
     lora_workspace_bytes, else allocated for the call."""
-    half, dev = (torch.bfloat16, torch.float16), x.device
-    if A.dim() != 3 or B.dim() != 3 or A.dtype not in half:
-        raise GlmMoeError("lora_add: expected A [adapters, r, K] and B [adapters, N, r], bf16 or fp16")
-    L, r, K = A.shape
-    N, n = B.shape[1], x.shape[0]
-    _need_on(A, A.dtype, L * r * K, "A", dev)
-    if tuple(B.shape) != (L, N, r):
-        raise GlmMoeError(f"B: expected [{L}, {N}, {r}]")
-    _need_on(B, A.dtype, L * N * r, "B", dev)
-    ldx = _need_rows(x, (torch.float32, A.dtype), n, K, "x")
-    _need_on(adapter_ids, torch.int32, n, "adapter_ids", dev)
-    ldb = _need_rows(base, (torch.float32, A.dtype), n, N, "base", dev)
-    ldy = _need_rows(y, (base.dtype,), n, N, "y", dev)
-    if scale is not None:
-        _need_on(scale, torch.float32, L, "scale", dev)
-    if ranks is not None:
-        _need_on(ranks, torch.int32, L, "ranks", dev)
-    with _on(dev):
-        if ws is None:
-            # On the stream that uses it, so that the allocator keeps it until then.
-            with _HERE if stream is None else torch.cuda.stream(stream):
-                ws = torch.empty(lora_workspace_bytes(n, L, K, r), dtype=torch.uint8, device=dev)
+    try:
+        (L, r, K), (LB, N, rB), (n, kx), idx, wt = A.shape, B.shape, x.shape, x.get_device(), A.dtype
+        (ldx, cx), (ldb, cb), (ldy, cy), xt, bt = x.stride(), base.stride(), y.stride(), x.dtype, base.dtype
+        ok = (idx >= 0 and kx == K and LB == L and rB == r and wt in _HALF and B.dtype == wt and xt in (wt, torch.float32)
+              and bt in (wt, torch.float32) and y.dtype == bt and A.is_contiguous() and B.is_contiguous()
+              and base.shape[0] >= n and y.shape[0] >= n and base.shape[1] == N and y.shape[1] == N
+              and (cx == 1 or K == 1) and ((cb == 1 and cy == 1) or N == 1)
+              and A.get_device() == idx and B.get_device() == idx and base.get_device() == idx and y.get_device() == idx
+              and adapter_ids.get_device() == idx and adapter_ids.dtype == torch.int32 and adapter_ids.is_contiguous()
+              and adapter_ids.numel() >= n)
+        if scale is not None:
+            ok = (ok and scale.get_device() == idx and scale.dtype == torch.float32 and scale.is_contiguous()
+                  and scale.numel() >= L)
+        if ranks is not None:
+            ok = (ok and ranks.get_device() == idx and ranks.dtype == torch.int32 and ranks.is_contiguous()
+                  and ranks.numel() >= L)
+        if ws is not None:
+            ok = ok and ws.get_device() == idx and ws.dtype == torch.uint8 and ws.is_contiguous()
+    except (AttributeError, TypeError, ValueError):
+        ok = False
+    if not ok:
+        _refuse_lora(x, adapter_ids, A, B, scale, base, y, ranks, ws)
+    if ws is None:
+        nb = lib().glmmoe_lora_workspace_bytes(n, L, K, r)
+        if stream is None:
+            ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
         else:
-            _need_on(ws, torch.uint8, 0, "ws", dev)
-        check(lib().glmmoe_lora_add(
-            _DTYPE[x.dtype], _p(x), ldx, _p(adapter_ids), n, _DTYPE[A.dtype], _p(A), _p(B), _p(ranks),
-            _p(scale), L, r, K, N, _DTYPE[y.dtype], _p(base), ldb, _p(y), ldy, _p(ws), ws.numel(),
-            _s(stream)), "lora_add")
+            with torch.cuda.stream(stream):   # so that the allocator keeps it until then
+                ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
+    _call(lib().glmmoe_lora_add, "lora_add", idx,
+          (_DTYPE[xt], x.data_ptr(), ldx if n > 1 else K, adapter_ids.data_ptr(), n, _DTYPE[wt], A.data_ptr(),
+           B.data_ptr(), None if ranks is None else ranks.data_ptr(), None if scale is None else scale.data_ptr(), L, r,
+           K, N, _DTYPE[bt], base.data_ptr(), ldb if n > 1 else N, y.data_ptr(), ldy if n > 1 else N, ws.data_ptr(),
+           ws.numel(), _stream_on(stream, idx)))
 
 
 def pack_fp8(w, n_mats, rows, K, out=None, stream=None):
