@@ -132,145 +132,6 @@ static long grid_items(const GroupedArgs& a, int tile_rows) {
     return (rows / tile_rows + (groups < rows ? groups : rows)) * a.ntn + 16 + kFewItems;
 }
 
-// Few rows per expert: the weights are streamed once and bound the time.
-// A workgroup has one tile of 16 TB rows and 16 NB rows of W (of each of the two
-// matrices where DUAL) over all of K; its 4 waves take chunks of 32 KS of K in
-// turn, straight from memory to registers, the next chunk's loads before this
-// chunk's products, and add their sums in LDS in order. W is the MFMA's A operand
-// (D row = output feature) and x its B (D column = row of the tile), so a lane
-// stores four consecutive features of one row. Columns past the tile's rows repeat
-// its first row and are dropped.
-constexpr int kStreamWaves = 4;
-
-template <class T, bool DUAL, int NB, int TB, int KS, bool AL, bool F32>
-__global__ __launch_bounds__(64 * kStreamWaves) void grp_stream_kernel(GroupedArgs a) {
-    constexpr int M = DUAL ? 2 : 1, LG = TB == 1 ? 4 : TB == 2 ? 5 : 6, KC = 32 * KS;
-    __shared__ f32x4 red[kStreamWaves][M * NB * TB][64];
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-    int e, r0, nr, col;
-    if (!find_item(a, LG, e, r0, nr, col)) return;
-    const uint16_t *w0 = a.w0 + (long)e * a.w_stride, *w1 = a.w1 + (long)e * a.w_stride;
-    if (e == a.E) w0 = a.s0, w1 = a.s1;
-    const int n0 = col * 16 * NB;
-    const int K = a.K;
-
-    const uint16_t* xp[TB];
-    bool ok[TB];
-#pragma unroll
-    for (int t = 0; t < TB; ++t) {
-        const int j = t * 16 + r, rr = j < nr ? r0 + j : r0;
-        const int id = a.row_ids ? a.row_ids[rr] : rr;
-        ok[t] = id >= 0 && id < a.x_rows;
-        xp[t] = a.x + (ok[t] ? (long)id : 0) * a.ldx;
-    }
-    const uint16_t* wp[M][NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const long at = (long)min(n0 + 16 * b + r, a.N - 1) * K;
-        wp[0][b] = w0 + at;
-        if constexpr (DUAL) wp[1][b] = w1 + at;
-    }
-
-    f32x4 acc[M][NB][TB];
-#pragma unroll
-    for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int t = 0; t < TB; ++t) acc[m][b][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-
-    struct Chunk {
-        u32x4 w[M][NB][KS], x[TB][KS];
-    };
-    auto load = [&](Chunk& c, int k0) {
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-#pragma unroll
-            for (int m = 0; m < M; ++m)
-#pragma unroll
-                for (int b = 0; b < NB; ++b) c.w[m][b][s] = load8<AL, AL>(wp[m][b], k0 + 32 * s + 8 * q);
-#pragma unroll
-            for (int t = 0; t < TB; ++t) c.x[t][s] = load8<AL>(xp[t], k0 + 32 * s + 8 * q);
-        }
-    };
-    auto mul = [&](const Chunk& c) {
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int m = 0; m < M; ++m)
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int t = 0; t < TB; ++t)
-                        acc[m][b][t] = T::mma(c.w[m][b][s], c.x[t][s], acc[m][b][t]);
-    };
-    constexpr int STEP = KC * kStreamWaves;
-    const int full = K / KC;                       // whole chunks; wave w takes w, w + 4, ...
-    int i = wv;
-    if (i < full) {
-        Chunk c0, c1;
-        load(c0, i * KC);
-        for (;;) {
-            i += kStreamWaves;
-            const bool more = i < full;
-            if (more) load(c1, i * KC);
-            mul(c0);
-            if (!more) break;
-            i += kStreamWaves;
-            const bool more2 = i < full;
-            if (more2) load(c0, i * KC);
-            mul(c1);
-            if (!more2) break;
-        }
-    }
-    if (full * KC < K && full % kStreamWaves == wv) {   // the rest of K, zeros after it
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int k = full * KC + 32 * s + 8 * q;
-            u32x4 x[TB];
-#pragma unroll
-            for (int t = 0; t < TB; ++t) x[t] = load8_tail<AL>(xp[t], k, K);
-#pragma unroll
-            for (int m = 0; m < M; ++m)
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const u32x4 w = load8_tail<AL>(wp[m][b], k, K);
-#pragma unroll
-                    for (int t = 0; t < TB; ++t) acc[m][b][t] = T::mma(w, x[t], acc[m][b][t]);
-                }
-        }
-    }
-
-#pragma unroll
-    for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int t = 0; t < TB; ++t) red[wv][(m * NB + b) * TB + t][lane] = acc[m][b][t];
-    __syncthreads();
-    auto total = [&](int f) {
-        f32x4 v = red[0][f][lane];
-#pragma unroll
-        for (int w = 1; w < kStreamWaves; ++w) v += red[w][f][lane];
-        return v;
-    };
-    for (int f = wv; f < NB * TB; f += kStreamWaves) {
-        const int b = f / TB, t = f % TB, j = t * 16 + r, n = n0 + 16 * b + 4 * q;
-        f32x4 v = total(f);
-        if constexpr (DUAL) {
-            const f32x4 u = total(NB * TB + f);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) v[c] = silu_fast(v[c]) * u[c];
-        }
-        bool good = true;
-#pragma unroll
-        for (int c = 0; c < TB; ++c) good = c == t ? ok[c] : good;
-        if (!good) v = (f32x4){0.f, 0.f, 0.f, 0.f};
-        if (j < nr && n < a.N)
-            store4<T, F32>(a.y, (long)(r0 + j) * a.ldy + n, v, a.N - n);
-    }
-}
-
 // Tiles of rows x TN rows of W (TN / 2 features of both matrices where DUAL), 64 of K per
 // step, D steps in LDS.
 //
@@ -283,7 +144,9 @@ __global__ __launch_bounds__(64 * kStreamWaves) void grp_stream_kernel(GroupedAr
 // barrier of a step stands before its last phase: behind it the next step is complete and this
 // step's LDS is free for the step D later.
 constexpr int kTileK = 64;
-template <class T, bool DUAL, bool F32, int WR, int WC, int NB, int LDS>
+// AL: rows of x and W are 16-byte aligned. Where they are not they come through registers, D = 2: loads of
+// step s + 2 are asked for behind the barrier of step s and go to LDS before the next one.
+template <class T, bool DUAL, bool F32, int WR, int WC, int NB, int LDS, bool AL = true>
 struct TileRun {
     static constexpr int W = WR * WC, TN = WC * NB * 16;
     const GroupedArgs& a;
@@ -294,7 +157,7 @@ struct TileRun {
     __device__ __forceinline__ void run() {
         constexpr int NP = MB > 4 ? 2 : 1, MH = (MB + NP - 1) / NP, PH = 2 * NP;
         constexpr int NA = MB * WR * 2, CA = (NA + W - 1) / W, CB = TN / 8 / W, BOFF = NA * 1024,
-                      STAGE = (NA + TN / 8) * 1024, D0 = LDS / STAGE, D = D0 < 8 ? D0 : 8;
+                      STAGE = (NA + TN / 8) * 1024, D0 = LDS / STAGE, D = !AL ? 2 : D0 < 8 ? D0 : 8;
         static_assert(D >= 2 && CB * W * 8 == TN, "two steps, whole instructions");
         const int r = lane & 15, q = lane >> 4, wr = wv / WC, wc = wv % WC;
         const int K = a.K, steps = (K + kTileK - 1) / kTileK;
@@ -341,15 +204,19 @@ struct TileRun {
             ids[i] = a.row_ids ? a.row_ids[rr] : rr;
             ka[i] = ((lane & 7) ^ (j >> 1 & 7)) * 8;
         }
+        if constexpr (AL) {
 #pragma unroll
-        for (int s = 0; s < D - 1; ++s)
-            if (s < steps) fetch_w(s, s * STAGE);
+            for (int s = 0; s < D - 1; ++s)
+                if (s < steps) fetch_w(s, s * STAGE);
+        }
 #pragma unroll
         for (int i = 0; i < CA; ++i)
             pa[i] = a.x + (ids[i] >= 0 && ids[i] < a.x_rows ? (long)ids[i] : 0) * a.ldx + ka[i];
+        if constexpr (AL) {
 #pragma unroll
-        for (int s = 0; s < D - 1; ++s)
-            if (s < steps) fetch_x(s, s * STAGE);
+            for (int s = 0; s < D - 1; ++s)
+                if (s < steps) fetch_x(s, s * STAGE);
+        }
         auto fetch = [&](int s, uint32_t stage) {
             const int k = s * kTileK;
             if (k + kTileK <= K) {
@@ -361,6 +228,23 @@ struct TileRun {
                 fetch_w(s, stage);
                 fetch_x(s, stage);
             }
+        };
+
+        u32x4 held[AL ? 1 : CA + CB];
+        auto grab = [&](int s) __attribute__((always_inline)) {
+            const int k = s * kTileK;
+#pragma unroll
+            for (int i = 0; i < CB; ++i) held[AL ? 0 : i] = load8_tail<false>(pb[i] - kb[i], k + kb[i], K);
+#pragma unroll
+            for (int i = 0; i < CA; ++i) held[AL ? 0 : CB + i] = load8_tail<false>(pa[i] - ka[i], k + ka[i], K);
+        };
+        auto drop = [&](uint32_t stage) __attribute__((always_inline)) {
+            char* p = lds + stage + lane * 16;
+#pragma unroll
+            for (int i = 0; i < CB; ++i)
+                *reinterpret_cast<u32x4*>(p + BOFF + (W * i + wv) * 1024) = held[AL ? 0 : i];
+#pragma unroll
+            for (int i = 0; i < CA; ++i) *reinterpret_cast<u32x4*>(p + at[i] * 1024) = held[AL ? 0 : CB + i];
         };
 
         f32x4 acc[MB][NB];
@@ -385,11 +269,21 @@ struct TileRun {
                     fb[kk][n] = *reinterpret_cast<const u32x4*>(rb + stage + c + n * 2048);
         };
 
-        if (steps >= D - 1) asm volatile("s_waitcnt vmcnt(%0)" :: "n"((D - 2) * CA) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        asm volatile("s_barrier" ::: "memory");
+        if constexpr (AL) {
+            if (steps >= D - 1) asm volatile("s_waitcnt vmcnt(%0)" :: "n"((D - 2) * CA) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            asm volatile("s_barrier" ::: "memory");
+        } else {
+            grab(0);
+            drop(0);
+            __syncthreads();
+        }
         read(0, 0);
-        if (D - 1 < steps) fetch(D - 1, (D - 1) * STAGE);
+        if constexpr (AL) {
+            if (D - 1 < steps) fetch(D - 1, (D - 1) * STAGE);
+        } else {
+            if (steps > 1) grab(1);
+        }
         uint32_t cur = 0;
         for (int s = 0; s < steps; ++s) {
 #pragma unroll
@@ -399,16 +293,23 @@ struct TileRun {
                 } else if (s + 1 < steps) {
                     // Step s + 1 has arrived, and this wave's reads of step s. What may be on its way then:
                     // D - 2 steps; before step D - 2, whose x was asked for after all the first W, less.
-                    if (s + D - 1 >= steps)
+                    if constexpr (!AL) {
+                        drop(cur ^ STAGE);      // all have read step s - 1, which was there
+                        __syncthreads();
+                    } else if (s + D - 1 >= steps) {
                         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n s_barrier" ::: "memory");
-                    else if (s < D - 3)
+                    } else if (s < D - 3) {
                         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n s_barrier" :: "n"((D - 2) * CA + CB) : "memory");
-                    else
+                    } else {
                         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n s_barrier" :: "n"((D - 2) * (CA + CB)) : "memory");
+                    }
                     const uint32_t free = cur;
                     cur = cur + STAGE == D * STAGE ? 0 : cur + STAGE;
                     read(cur, 0);
-                    if (s + D < steps) fetch(s + D, free);
+                    if (s + D < steps) {
+                        if constexpr (AL) fetch(s + D, free);
+                        else grab(s + D);
+                    }
                 }
                 const int kk = p / NP, h = p % NP;
 #pragma unroll
@@ -476,6 +377,18 @@ __global__ __launch_bounds__(256, 2) void grp_slim_kernel(GroupedArgs a) {
     else t.template run<4>();
 }
 
+// Rows at any address: up to 64 rows x 128 rows of W, three workgroups of 4 waves to a CU.
+template <class T, bool DUAL, bool F32>
+__global__ __launch_bounds__(256, 3) void grp_any_kernel(GroupedArgs a) {
+    __shared__ __align__(16) char lds[48 * 1024];
+    TileRun<T, DUAL, F32, 1, 4, 2, 48 * 1024, false> t{a, lds, 0, 0, 0, 0, (int)(threadIdx.x & 63),
+                                                       __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)};
+    if (!find_item(a, 6, t.e, t.r0, t.nr, t.col)) return;
+    if (t.nr <= 16) t.template run<1>();
+    else if (t.nr <= 32) t.template run<2>();
+    else t.template run<4>();
+}
+
 // Rows per expert up to which the slim kernel runs: gate and up, 6144 -> 2048, 256 experts, at 16 / 32 / 64
 // rows each 2.08 / 2.10 / 3.06 ms against the large kernel's 2.06 / 2.10 / 2.16; at 2 rows 1.83 and
 // 1.95, with 256 features of the 32-row groups of a skewed router 0.294 and 0.361.
@@ -488,32 +401,18 @@ static long mean_rows(const GroupedArgs& a) {
 }
 
 template <class T, bool DUAL, bool F32>
-static int run_tiles(const GroupedArgs& a0, hipStream_t s) {
+static int run_tiles(const GroupedArgs& a0, bool aligned, hipStream_t s) {
     GroupedArgs a = a0;
-    const bool slim = mean_rows(a) <= kSlimRows;
-    const int w = (slim ? 128 : 256) / (DUAL ? 2 : 1);
+    const bool slim = mean_rows(a) <= kSlimRows, large = aligned && !slim;
+    const int w = (large ? 256 : 128) / (DUAL ? 2 : 1);
     a.ntn = (a.N + w - 1) / w;
     a.fours = mean_rows(a) > 256;                // fewer: an expert's W belongs to one tile
-    const long grid = grid_items(a, slim ? 64 : 256);
-    if (grid >= (1L << 31)) return -2;
-    if (slim) hipLaunchKernelGGL((grp_slim_kernel<T, DUAL, F32>), dim3((unsigned)grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((grp_tile_kernel<T, DUAL, F32>), dim3((unsigned)grid), dim3(512), 0, s, a);
-    return hipGetLastError() == hipSuccess ? 0 : -4;
-}
-
-template <class T, bool DUAL, bool F32>
-static int run_stream(const GroupedArgs& a0, hipStream_t s) {
-    GroupedArgs a = a0;
-    const long mean = mean_rows(a);
-    const int tb = mean <= 16 ? 1 : mean <= 32 ? 2 : 4;
-    constexpr int NB = DUAL ? 1 : 2;
-    a.ntn = (a.N + 16 * NB - 1) / (16 * NB);
-    const long grid = grid_items(a, 16 * tb);
-    if (grid >= (1L << 31)) return -2;
-    const dim3 g((unsigned)grid), b(64 * kStreamWaves);
-    if (tb == 1) hipLaunchKernelGGL((grp_stream_kernel<T, DUAL, NB, 1, 4, false, F32>), g, b, 0, s, a);
-    else if (tb == 2) hipLaunchKernelGGL((grp_stream_kernel<T, DUAL, NB, 2, 4, false, F32>), g, b, 0, s, a);
-    else hipLaunchKernelGGL((grp_stream_kernel<T, DUAL, NB, 4, 2, false, F32>), g, b, 0, s, a);
+    const long items = grid_items(a, large ? 256 : 64);
+    if (items >= (1L << 31)) return -2;
+    const dim3 grid((unsigned)items);
+    if (large) hipLaunchKernelGGL((grp_tile_kernel<T, DUAL, F32>), grid, dim3(512), 0, s, a);
+    else if (aligned) hipLaunchKernelGGL((grp_slim_kernel<T, DUAL, F32>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((grp_any_kernel<T, DUAL, F32>), grid, dim3(256), 0, s, a);
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }
 
@@ -566,8 +465,7 @@ static int run_types(const GroupedArgs& a, bool f32, hipStream_t s) {
     auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     const bool aligned = a.K % 8 == 0 && a.ldx % 8 == 0 && a.w_stride % 8 == 0 && al(a.x) &&
                          al(a.w0) && (!DUAL || al(a.w1)) && al(a.s0) && al(a.s1);
-    if (aligned) return f32 ? run_tiles<T, DUAL, true>(a, s) : run_tiles<T, DUAL, false>(a, s);
-    return f32 ? run_stream<T, DUAL, true>(a, s) : run_stream<T, DUAL, false>(a, s);
+    return f32 ? run_tiles<T, DUAL, true>(a, aligned, s) : run_tiles<T, DUAL, false>(a, aligned, s);
 }
 
 int launch_grouped(const GroupedArgs& a, int dtype, bool f32, hipStream_t s) {
