@@ -194,8 +194,11 @@ def run(state):
         elif op == "gate_up":
             G.grouped_gate_up(state["x"], state["w"], state["up"], state["offsets"], state["y"], state["rows"])
         else:
-            G.lora_add(state["x"], state["ids"], state["A"], state["B"], state["scale"], state["base"], state["y"],
-                       ranks=state["ranks"])
+            # fp32 rows are added to in place, as the plain form does; 16-bit ones go to a buffer of their own.
+            base = state["base"]
+            y = base if base.dtype == torch.float32 else state["y"]
+            G.lora_add(state["x"], state["ids"], state["A"], state["B"], state["scale"], base, y, ranks=state["ranks"])
+            return y
         return state["y"]
     if op == "lora":
         return _plain_lora(state)
