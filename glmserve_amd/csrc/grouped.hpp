@@ -43,7 +43,7 @@ struct LoraArgs {
     long ldy;
     float* part;              // lora_part_bytes: [splits][n][rp], A x of each K split
     int splits, kstep, rp;    // set by the launch: K per split, row length of part,
-    int jn, nx;               // workgroups per token block (by adapter), along N
+    int jm, je, nx;           // workgroups per token block (by adapter), at both ends; along N
 };
 size_t lora_part_bytes(int n, int L, int K, int r);
 int launch_lora(const LoraArgs& a, int xdt, int wdt, int ydt, hipStream_t s);

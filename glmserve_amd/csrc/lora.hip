@@ -138,6 +138,41 @@ struct XFloat {         // x fp32
     static __device__ __forceinline__ f32x4 mma(u32x4 w, const Terms3& x, f32x4 c) { return mma3<W>(w, x, c); }
 };
 
+// What a workgroup does of the tokens' blocks (16 TB tokens each): the j-th adapter of a block and every
+// jn-th after it. The workgroups that few blocks need come first, so that those that all blocks need
+// fill all XCDs (id % 8) evenly: a batch of prompts has one adapter in a block, but where its decoding
+// requests stand, before or after them, a block has many, so the blocks of the first and last
+// 64 tokens have je workgroups, the others jm. Blocks go from the last to the first.
+constexpr int kEndTokens = 64;
+template <int TB>
+struct BlockItem {
+    int t0, j, jn;
+    static __host__ __device__ __forceinline__ int blocks(int n) { return (n + 16 * TB - 1) / (16 * TB); }
+    static __host__ __device__ __forceinline__ int ends(int n) {
+        const int both = 2 * kEndTokens / (16 * TB), b = blocks(n);
+        return b < both ? b : both;
+    }
+    static __host__ __forceinline__ long count(const LoraArgs& a) {
+        return (long)blocks(a.n) * a.jm + (long)ends(a.n) * (a.je - a.jm);
+    }
+    __device__ __forceinline__ BlockItem(const LoraArgs& a, int id) {
+        constexpr int EB = kEndTokens / (16 * TB);
+        const int nb = blocks(a.n), ne = ends(a.n), more = a.je - a.jm;
+        int b;
+        if (id < ne * more) {
+            const int e = id / more;
+            b = e < EB ? e : nb - ne + e;
+            j = a.jm + id % more;
+        } else {
+            id -= ne * more;
+            b = nb - 1 - id % nb;
+            j = a.jm - 1 - id / nb;
+        }
+        t0 = b * 16 * TB;
+        jn = b < EB || b >= nb - (ne - EB) ? a.je : a.jm;
+    }
+};
+
 // The adapters of a block of tokens, one after the other, every jn-th from the j-th on.
 struct Adapters {
     int id;                   // lane i: its token's adapter, -1 for none
@@ -166,11 +201,9 @@ __device__ __forceinline__ int rank_of(const LoraArgs& a, int ad) {
 }
 
 // part[split][t][:] = A[ids[t]][:, K of the split] x[t][K of the split]. A workgroup: 16 TB
-// tokens, 16 RB ranks, one split, every jn-th adapter of the block: the workgroups of the last j, few
-// of which find an adapter, come first, so that the others fill all XCDs (id % 8) evenly. A is the
-// MFMA's A operand (D row = rank), x its B (D column = token).
+// tokens, 16 RB ranks, one split. A is the MFMA's A operand (D row = rank), x its B (D column = token).
 struct DownItem {
-    int split, rank0, j, t0, kb, ke;
+    int split, rank0, j, jn, t0, kb, ke;
     template <int RB, int TB>
     static __device__ __forceinline__ DownItem of(const LoraArgs& a) {
         DownItem d;
@@ -180,9 +213,8 @@ struct DownItem {
         const int rg = a.rp / 16 > RB ? (a.rp / 16 + RB - 1) / RB : 1;
         d.rank0 = id % rg * RB * 16;
         id /= rg;
-        const int blocks = (a.n + 16 * TB - 1) / (16 * TB);
-        d.j = a.jn - 1 - id / blocks;
-        d.t0 = (blocks - 1 - id % blocks) * 16 * TB;
+        const BlockItem<TB> b(a, id);
+        d.t0 = b.t0, d.j = b.j, d.jn = b.jn;
         d.kb = d.split * a.kstep;
         d.ke = min(a.K, d.kb + a.kstep);
         return d;
@@ -231,7 +263,7 @@ __global__ __launch_bounds__(64 * kLoraWaves, 2) void lora_down_kernel(LoraArgs 
     Adapters list(block_id(a, t0, 16 * TB), j);
     int ad;
     uint64_t m;
-    while (list.next(a.jn, ad, m)) {
+    while (list.next(d.jn, ad, m)) {
         const int rk = rank_of(a, ad);
         f32x4 acc[RB][TB];
         const uint16_t* wp[RB];
@@ -333,7 +365,7 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 2 : 1) void lora_down_ri
     Adapters list(block_id(a, d.t0, XR), d.j);
     int ad;
     uint64_t m;
-    while (list.next(a.jn, ad, m)) {
+    while (list.next(d.jn, ad, m)) {
         const int rk = rank_of(a, ad);
         f32x4 acc[RB][TB];
 #pragma unroll
@@ -444,18 +476,11 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 4 : 2) void lora_up_kern
     int id = blockIdx.x;
     const int n0 = (id % a.nx * kLoraWaves + wv) * 16 * NB;
     id /= a.nx;
-    const int blocks = (a.n + 16 * TB - 1) / (16 * TB);
-    const int j = a.jn - 1 - id / blocks, t0 = (blocks - 1 - id % blocks) * 16 * TB;   // as in the first launch
-    const int ad0 = block_id(a, t0, 16 * TB);
-    const uint64_t has = __ballot(ad0 >= 0);
-    Adapters list(ad0, j);
-    int ad;
-    uint64_t m;
-    bool some = list.next(a.jn, ad, m);
+    const BlockItem<TB> item(a, id);
+    const int j = item.j, jn = item.jn, t0 = item.t0;
     const int left = min(a.n - t0, 16 * TB);
-    // Tokens without an adapter are copied; in place they are there already.
-    const uint64_t none = j == 0 && a.y != a.base ? ~has & (left >= 64 ? ~0ull : (1ull << left) - 1) : 0;
-    if (!some && !none) return;
+    const uint64_t here = left >= 64 ? ~0ull : (1ull << left) - 1;
+    const int id0 = lane < left ? a.ids[t0 + lane] : -1;
 
     const int n4 = a.N & ~3, nl = n0 + 4 * q;                    // whole fours; the lane's first column
     const elem* pb = static_cast<const elem*>(a.base) + (long)(t0 + r) * a.ldb + nl;
@@ -486,38 +511,58 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 4 : 2) void lora_up_kern
                     if (nl + 16 * b < n4) base[t][b] = O::get4(p + 16 * b);
             }
     };
+    // The workgroups that all blocks have ask for the block's base and A x before they know its adapters.
+    const int segs = stride / 8, tasks = 16 * TB * segs;
+    const long step = (long)a.n * a.rp;
+    auto load_part = [&](f32x4 (&u)[4][2], int i, int s) __attribute__((always_inline)) {
+        const int t = min(i / segs, left - 1), k = min(i % segs * 8, a.rp - 8);
+        const float* p = a.part + (long)(t0 + t) * a.rp + k;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            const float* ps = p + min(s + d, a.splits - 1) * step;
+            u[d][0] = *reinterpret_cast<const f32x4*>(ps);
+            u[d][1] = *reinterpret_cast<const f32x4*>(ps + 4);
+        }
+    };
+    f32x4 u[4][2];
+    if (j == 0) {
+        load_base(here);
+        load_part(u, min((int)threadIdx.x, tasks - 1), 0);
+    }
+    const int ad0 = id0 >= 0 && id0 < a.L ? id0 : -1;
+    const uint64_t has = __ballot(ad0 >= 0);
+    Adapters list(ad0, j);
+    int ad;
+    uint64_t m;
+    bool some = list.next(jn, ad, m);
+    // Tokens without an adapter are copied; in place they are there already.
+    const uint64_t none = j == 0 && a.y != a.base ? ~has & here : 0;
+    if (!some && !none) return;
     auto begin = [&]() __attribute__((always_inline)) {
         rk = rank_of(a, ad);
 #pragma unroll
         for (int b = 0; b < NB; ++b) wp[b] = a.B + ((long)ad * a.N + min(n0 + 16 * b + r, a.N - 1)) * a.r;
         load_w(0);
-        load_base(m);
+        if (j != 0) load_base(m);
     };
     if (some) begin();
 
-    const int segs = stride / 8;
-    for (int i = threadIdx.x; i < 16 * TB * segs; i += 64 * kLoraWaves) {
+    for (int i = threadIdx.x; i < tasks; i += 64 * kLoraWaves) {
         const int t = i / segs, k = i % segs * 8;
         float v[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) v[c] = 0.0f;
-        if (k < a.rp && (has >> t & 1)) {
-            const float* p = a.part + (long)(t0 + t) * a.rp + k;
-            const long step = (long)a.n * a.rp;
-            for (int s = 0; s < a.splits; s += 4) {
-                f32x4 u[4][2];
+        for (int s = 0; s < a.splits; s += 4) {
+            if (j != 0 || s > 0 || i >= 64 * kLoraWaves) load_part(u, i, s);
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const float* ps = p + min(s + d, a.splits - 1) * step;
-                    u[d][0] = *reinterpret_cast<const f32x4*>(ps);
-                    u[d][1] = *reinterpret_cast<const f32x4*>(ps + 4);
-                }
+            for (int d = 0; d < 4; ++d)
 #pragma unroll
-                for (int d = 0; d < 4; ++d)
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) v[c] = s + d < a.splits ? v[c] + u[d][c / 4][c % 4] : v[c];
-            }
+                for (int c = 0; c < 8; ++c) v[c] = s + d < a.splits ? v[c] + u[d][c / 4][c % 4] : v[c];
         }
+        // Rows of tokens without an adapter, and what lies past the ranks, hold nothing.
+        const bool live = k < a.rp && (has >> t & 1);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = live ? v[c] : 0.0f;
         const Terms3 o = split3(v);
 #pragma unroll
         for (int c = 0; c < 3; ++c) *reinterpret_cast<u32x4*>(terms + (c * 16 * TB + t) * stride + k) = o.t[c];
@@ -569,11 +614,10 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 4 : 2) void lora_up_kern
                 const elem* p = static_cast<const elem*>(a.base) + (long)(t0 + lane) * a.ldb + n;
                 O::put(static_cast<elem*>(a.y) + (long)(t0 + lane) * a.ldy + n, __builtin_fmaf(sc, v, O::get(p)));
             }
-        some = list.next(a.jn, ad, m);
+        some = list.next(jn, ad, m);
         if (some) begin();
     }
     if (none) {
-        load_base(none);
 #pragma unroll
         for (int t = 0; t < TB; ++t)
             if (none >> (16 * t + r) & 1) {
@@ -589,23 +633,24 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 4 : 2) void lora_up_kern
     }
 }
 
-// How the first launch splits K: 512 workgroups (with 256 / 1024 the case above takes 125 / 110 us), 512 of
-// K at least.
+// How the first launch splits K: into 512 workgroups (256 and 1024 of them: 4096 tokens as above 75 and 110 us
+// against 71, 64 decoding tokens of 32 adapters 22.5 and 26.7 against 23.5), 512 of K at least.
 struct LoraPlan {
-    int tb, blocks, jn, splits, kstep, rp;
+    int tb, jm, je, splits, kstep, rp;
 };
 static LoraPlan plan_of(int n, int L, int K, int r) {
     LoraPlan p;
     p.tb = n > 1024 ? 2 : 1;
-    p.blocks = (n + 16 * p.tb - 1) / (16 * p.tb);
     const int most = n < L ? n : L;
-    // Workgroups per block of tokens, over its adapters: a batch of decoding tokens has up to 16 in a
-    // block, a long one is mostly prompts with one, and a workgroup that finds no adapter costs its
-    // start (4096 tokens of 8 prompts and 32 decoding tokens: 146 / 85 / 87 us with 1 / 2 / 4).
-    const int jn = n <= 1024 ? 16 : n <= 8192 ? 2 : 1;
-    p.jn = most < jn ? most : jn;
+    // A workgroup that finds no adapter costs its start: up to 256 tokens may all be decoding, beyond
+    // most are prompts' (4096 tokens of 8 prompts and 32 decoding tokens at the end, rank 64, fp32 6144 ->
+    // 2048: 146 us with one workgroup for every block, 85 with two, 72 with two and 16 at the ends; 700 tokens
+    // of 3 prompts and 32: 22 with 16 for every block, 18 so).
+    const int jm = n <= 256 ? 16 : n <= 1024 ? 4 : 2;
+    p.je = most < 16 ? most : 16;
+    p.jm = p.je < jm ? p.je : jm;
     p.rp = (r + 15) / 16 * 16;
-    const long wgs = (long)p.blocks * (n <= 256 ? p.jn : 1) * ((r + 16 * kRankBlocks - 1) / (16 * kRankBlocks));
+    const long wgs = (long)((n + 16 * p.tb - 1) / (16 * p.tb)) * (n <= 256 ? p.jm : 1) * ((r + 16 * kRankBlocks - 1) / (16 * kRankBlocks));
     long s = (512 + wgs - 1) / wgs;
     const int top = (K + 511) / 512;
     s = s < 1 ? 1 : s > top ? top : s;
@@ -639,25 +684,25 @@ static void run_down(const LoraArgs& a, const LoraPlan& p, bool aligned, unsigne
 template <class W, int YD>
 static int run_up(const LoraArgs& a0, hipStream_t s) {
     LoraArgs a = a0;
-    const int tb = a.n > 1024 && a.r <= 128 ? 4 : 1;   // 52 KiB of LDS at most
-    const long blocks = (a.n + 16 * tb - 1) / (16 * tb);
+    const int tb = a.n > 1024 ? 2 : 1;
     a.nx = (a.N + 255) / 256;
-    const long grid = blocks * a.jn * a.nx;
+    const long grid = (tb == 1 ? BlockItem<1>::count(a) : BlockItem<2>::count(a)) * a.nx;
     if (grid >= (1L << 31)) return -2;
     const size_t lds = (size_t)3 * 16 * tb * ((a.r + 31) / 32 * 32 + 8) * 2;
     const dim3 g((unsigned)grid), b(64 * kLoraWaves);
     if (tb == 1) hipLaunchKernelGGL((lora_up_kernel<W, YD, 1>), g, b, lds, s, a);
-    else hipLaunchKernelGGL((lora_up_kernel<W, YD, 4>), g, b, lds, s, a);
+    else hipLaunchKernelGGL((lora_up_kernel<W, YD, 2>), g, b, lds, s, a);
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }
 
 int launch_lora(const LoraArgs& a0, int xdt, int wdt, int ydt, hipStream_t s) {
     LoraArgs a = a0;
     const LoraPlan p = plan_of(a.n, a.L, a.K, a.r);
-    a.splits = p.splits, a.kstep = p.kstep, a.rp = p.rp, a.jn = p.jn;
+    a.splits = p.splits, a.kstep = p.kstep, a.rp = p.rp, a.jm = p.jm, a.je = p.je;
     auto al = [](const void* q, size_t v) { return reinterpret_cast<uintptr_t>(q) % v == 0; };
     const bool aligned = a.K % 8 == 0 && al(a.x, 16) && al(a.A, 16) && a.ldx % (xdt == kF32 ? 4 : 8) == 0;
-    const long grid = (long)p.blocks * p.jn * ((p.rp / 16 + kRankBlocks - 1) / kRankBlocks) * p.splits;
+    const long grid = (p.tb == 1 ? BlockItem<1>::count(a) : BlockItem<2>::count(a)) *
+                      ((p.rp / 16 + kRankBlocks - 1) / kRankBlocks) * p.splits;
     if (grid >= (1L << 31)) return -2;
     auto down = [&](auto w) {
         using W = decltype(w);
