@@ -144,9 +144,11 @@ static long grid_items(const GroupedArgs& a, int tile_rows) {
 // barrier of a step stands before its last phase: behind it the next step is complete and this
 // step's LDS is free for the step D later.
 constexpr int kTileK = 64;
+// NT: W is read without a place in L2, where no other tile wants it (64 tokens of 8 of 256 experts, gate and
+// up 6144 -> 2048: 1837 -> 1680 us, 6.7 TB/s; but 8192 rows of one expert, 8192 -> 8192, 869 -> 919).
 // AL: rows of x and W are 16-byte aligned. Where they are not they come through registers, D = 2: loads of
 // step s + 2 are asked for behind the barrier of step s and go to LDS before the next one.
-template <class T, bool DUAL, bool F32, int WR, int WC, int NB, int LDS, bool AL = true>
+template <class T, bool DUAL, bool F32, int WR, int WC, int NB, int LDS, bool NT, bool AL = true>
 struct TileRun {
     static constexpr int W = WR * WC, TN = WC * NB * 16;
     const GroupedArgs& a;
@@ -177,7 +179,7 @@ struct TileRun {
             const bool whole = k + kTileK <= K;
 #pragma unroll
             for (int i = 0; i < CB; ++i)
-                copy16(whole || k + kb[i] < K ? static_cast<const void*>(pb[i] + k) : &kZero16,
+                copy16<NT>(whole || k + kb[i] < K ? static_cast<const void*>(pb[i] + k) : &kZero16,
                        la + stage + BOFF + (W * i + wv) * 1024);
         };
         auto fetch_x = [&](int s, uint32_t stage) {
@@ -221,7 +223,7 @@ struct TileRun {
             const int k = s * kTileK;
             if (k + kTileK <= K) {
 #pragma unroll
-                for (int i = 0; i < CB; ++i) copy16(pb[i] + k, la + stage + BOFF + (W * i + wv) * 1024);
+                for (int i = 0; i < CB; ++i) copy16<NT>(pb[i] + k, la + stage + BOFF + (W * i + wv) * 1024);
 #pragma unroll
                 for (int i = 0; i < CA; ++i) copy16(pa[i] + k, la + stage + at[i] * 1024);
             } else {
@@ -346,15 +348,15 @@ struct TileRun {
 };
 
 // Up to 256 rows x 256 rows of W, one workgroup of 8 waves to a CU.
-template <class T, bool DUAL, bool F32>
+template <class T, bool DUAL, bool F32, bool NT>
 __global__ __launch_bounds__(512, 2) void grp_tile_kernel(GroupedArgs a) {
     __shared__ __align__(16) char lds[160 * 1024];
-    TileRun<T, DUAL, F32, 2, 4, 4, 160 * 1024> t{a, lds, 0, 0, 0, 0, (int)(threadIdx.x & 63),
+    TileRun<T, DUAL, F32, 2, 4, 4, 160 * 1024, NT> t{a, lds, 0, 0, 0, 0, (int)(threadIdx.x & 63),
                                                  __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)};
     int halves;
     if (!find_item(a, 8, t.e, t.r0, t.nr, t.col, &halves)) return;
     if (halves) {
-        TileRun<T, DUAL, F32, 2, 4, 2, 160 * 1024> h{a, lds, t.e, t.r0, t.nr, t.col, t.lane, t.wv};
+        TileRun<T, DUAL, F32, 2, 4, 2, 160 * 1024, NT> h{a, lds, t.e, t.r0, t.nr, t.col, t.lane, t.wv};
         if (t.nr <= 32) h.template run<1>();
         else if (t.nr <= 64) h.template run<2>();
         else h.template run<4>();
@@ -369,7 +371,7 @@ __global__ __launch_bounds__(512, 2) void grp_tile_kernel(GroupedArgs a) {
 template <class T, bool DUAL, bool F32>
 __global__ __launch_bounds__(256, 2) void grp_slim_kernel(GroupedArgs a) {
     __shared__ __align__(16) char lds[80 * 1024];
-    TileRun<T, DUAL, F32, 1, 4, 2, 80 * 1024> t{a, lds, 0, 0, 0, 0, (int)(threadIdx.x & 63),
+    TileRun<T, DUAL, F32, 1, 4, 2, 80 * 1024, true> t{a, lds, 0, 0, 0, 0, (int)(threadIdx.x & 63),
                                                 __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)};
     if (!find_item(a, 6, t.e, t.r0, t.nr, t.col)) return;
     if (t.nr <= 16) t.template run<1>();
@@ -381,7 +383,7 @@ __global__ __launch_bounds__(256, 2) void grp_slim_kernel(GroupedArgs a) {
 template <class T, bool DUAL, bool F32>
 __global__ __launch_bounds__(256, 3) void grp_any_kernel(GroupedArgs a) {
     __shared__ __align__(16) char lds[48 * 1024];
-    TileRun<T, DUAL, F32, 1, 4, 2, 48 * 1024, false> t{a, lds, 0, 0, 0, 0, (int)(threadIdx.x & 63),
+    TileRun<T, DUAL, F32, 1, 4, 2, 48 * 1024, false, false> t{a, lds, 0, 0, 0, 0, (int)(threadIdx.x & 63),
                                                        __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)};
     if (!find_item(a, 6, t.e, t.r0, t.nr, t.col)) return;
     if (t.nr <= 16) t.template run<1>();
@@ -390,8 +392,8 @@ __global__ __launch_bounds__(256, 3) void grp_any_kernel(GroupedArgs a) {
 }
 
 // Rows per expert up to which the slim kernel runs: gate and up, 6144 -> 2048, 256 experts, at 16 / 32 / 64
-// rows each 2.08 / 2.10 / 3.06 ms against the large kernel's 2.06 / 2.10 / 2.16; at 2 rows 1.83 and
-// 1.95, with 256 features of the 32-row groups of a skewed router 0.294 and 0.361.
+// rows each 1.88 / 1.94 / 3.04 ms against the large kernel's 1.96 / 1.99 / 2.05; with 256 features and a skewed
+// router (32 rows on average) 0.30 against 0.32.
 constexpr int kSlimRows = 40;
 
 // Rows per expert, on average over the experts that can have any.
@@ -406,11 +408,13 @@ static int run_tiles(const GroupedArgs& a0, bool aligned, hipStream_t s) {
     const bool slim = mean_rows(a) <= kSlimRows, large = aligned && !slim;
     const int w = (large ? 256 : 128) / (DUAL ? 2 : 1);
     a.ntn = (a.N + w - 1) / w;
-    a.fours = mean_rows(a) > 256;                // fewer: an expert's W belongs to one tile
+    // More rows: the tiles of an expert share its W. Fewer: W is read once and keeps out of L2.
+    a.fours = mean_rows(a) > 256;
     const long items = grid_items(a, large ? 256 : 64);
-    if (items >= (1L << 31)) return -2;
+    if (items * 512 >= (1L << 32)) return -2;     // threads of a launch
     const dim3 grid((unsigned)items);
-    if (large) hipLaunchKernelGGL((grp_tile_kernel<T, DUAL, F32>), grid, dim3(512), 0, s, a);
+    if (large && a.fours) hipLaunchKernelGGL((grp_tile_kernel<T, DUAL, F32, false>), grid, dim3(512), 0, s, a);
+    else if (large) hipLaunchKernelGGL((grp_tile_kernel<T, DUAL, F32, true>), grid, dim3(512), 0, s, a);
     else if (aligned) hipLaunchKernelGGL((grp_slim_kernel<T, DUAL, F32>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((grp_any_kernel<T, DUAL, F32>), grid, dim3(256), 0, s, a);
     return hipGetLastError() == hipSuccess ? 0 : -4;
@@ -454,7 +458,7 @@ __global__ __launch_bounds__(256) void grp_combine_kernel(const float* __restric
 int launch_grouped_combine(const float* part, const int* inv, const int* ids, const float* w, int n,
                            int topk, int E, int H, int shared, float* out, hipStream_t s) {
     const long grid = (long)n * ((H / 4 + 255) / 256);
-    if (H % 4 || topk > 8 || grid >= (1L << 31)) return -2;
+    if (H % 4 || topk > 8 || grid * 256 >= (1L << 32)) return -2;
     hipLaunchKernelGGL(grp_combine_kernel, dim3((unsigned)grid), dim3(256), 0, s, part, inv, ids, w,
                        n, topk, E, H, shared, out);
     return hipGetLastError() == hipSuccess ? 0 : -4;

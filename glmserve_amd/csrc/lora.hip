@@ -687,7 +687,7 @@ static int run_up(const LoraArgs& a0, hipStream_t s) {
     const int tb = a.n > 1024 ? 2 : 1;
     a.nx = (a.N + 255) / 256;
     const long grid = (tb == 1 ? BlockItem<1>::count(a) : BlockItem<2>::count(a)) * a.nx;
-    if (grid >= (1L << 31)) return -2;
+    if (grid * 64 * kLoraWaves >= (1L << 32)) return -2;   // threads of a launch
     const size_t lds = (size_t)3 * 16 * tb * ((a.r + 31) / 32 * 32 + 8) * 2;
     const dim3 g((unsigned)grid), b(64 * kLoraWaves);
     if (tb == 1) hipLaunchKernelGGL((lora_up_kernel<W, YD, 1>), g, b, lds, s, a);
@@ -703,7 +703,7 @@ int launch_lora(const LoraArgs& a0, int xdt, int wdt, int ydt, hipStream_t s) {
     const bool aligned = a.K % 8 == 0 && al(a.x, 16) && al(a.A, 16) && a.ldx % (xdt == kF32 ? 4 : 8) == 0;
     const long grid = (p.tb == 1 ? BlockItem<1>::count(a) : BlockItem<2>::count(a)) *
                       ((p.rp / 16 + kRankBlocks - 1) / kRankBlocks) * p.splits;
-    if (grid >= (1L << 31)) return -2;
+    if (grid * 64 * kLoraWaves >= (1L << 32)) return -2;   // threads of a launch
     auto down = [&](auto w) {
         using W = decltype(w);
         const unsigned g = (unsigned)grid;

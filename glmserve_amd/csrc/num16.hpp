@@ -79,9 +79,15 @@ static __device__ const u32x4 kZero16 = {0u, 0u, 0u, 0u};
 
 // 64 lanes x 16 B from memory to LDS at base + 16 * lane, without the compiler's knowledge: it
 // would have every LDS read wait for all of them.
+// NT: read once, not worth a place in L2.
+template <bool NT = false>
 __device__ __forceinline__ void copy16(const void* g, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n s_nop 0\n global_load_lds_dwordx4 %0, off"
-                 :: "v"(g), "s"(lds) : "memory");
+    if constexpr (NT)
+        asm volatile("s_mov_b32 m0, %1\n s_nop 0\n global_load_lds_dwordx4 %0, off nt"
+                     :: "v"(g), "s"(lds) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %1\n s_nop 0\n global_load_lds_dwordx4 %0, off"
+                     :: "v"(g), "s"(lds) : "memory");
 }
 
 // Four consecutive outputs of a row from element `at` on, of which cnt are inside it.

@@ -319,8 +319,10 @@ int glmmoe_expert_ffn_fp8(const glmmoe_fp8_layer* L, const uint16_t* x, int n,
  *                   outside [0, rows] are taken as the nearest of the two
  *   y, y_dtype, ldy [rows, N], rows ldy apart; GLMMOE_F32, or dtype
  * Any N and K; K, ldx and w_stride multiples of 8 with 16-byte aligned x and w are read
- * in whole vectors. y must not overlap x. rows == 0 returns GLMMOE_OK. No workspace.
- * Limits: E <= 4096, rows and x_rows < 2^30, K and N < 2^24. */
+ * in whole vectors. y must not overlap x. rows == 0 returns GLMMOE_OK. No workspace. bf16
+ * values below 2^-126 count as zero (the matrix cores take them so), fp16 ones do not.
+ * Limits: E <= 4096, rows and x_rows < 2^30, K and N < 2^24, rows x N within what one
+ * launch's tiles cover (GLMMOE_ERR_SHAPE beyond: 2^23 tiles of 64 x 128 and more). */
 int glmmoe_grouped_linear(int dtype, const void* x, int64_t ldx, int64_t x_rows,
                           const int* row_ids, const void* w, int64_t w_stride,
                           const int* expert_offsets, int E, int64_t rows, int64_t N, int64_t K,
@@ -351,8 +353,9 @@ int glmmoe_grouped_gate_up(int dtype, const void* x, int64_t ldx, int64_t x_rows
  * bits). One rounding, to y's type. Sums run in a fixed order.
  * Tokens of a request are expected to be neighbours: 16 to 64 consecutive tokens share
  * the weights of each adapter that occurs among them.
- * Workspace: glmmoe_lora_workspace_bytes (A x; 0 for arguments out of range). n == 0
- * returns GLMMOE_OK. Limits: r <= 256, n < 2^24, K and N < 2^24. */
+ * Workspace: glmmoe_lora_workspace_bytes (A x; 0 for arguments out of range), 16-byte
+ * aligned; calls that may overlap need one each. n == 0 returns GLMMOE_OK. Limits:
+ * r <= 256, n < 2^24, n_adapters <= 2^24, K and N < 2^24. */
 size_t glmmoe_lora_workspace_bytes(int n, int n_adapters, int64_t K, int r);
 int glmmoe_lora_add(int x_dtype, const void* x, int64_t ldx, const int* adapter_ids, int n,
                     int w_dtype, const void* A, const void* B, const int* ranks,

@@ -57,7 +57,7 @@ def _check(out, want):
 
 
 @pytest.mark.parametrize("H,I,E,k,shared", [(256, 128, 16, 4, True), (512, 200, 40, 8, False),
-                                            (768, 256, 300, 8, True)])
+                                            (768, 256, 300, 8, True), (256, 64, 512, 8, True)])
 @pytest.mark.parametrize("n", [1, 7, 64, 300, 1200])
 def test_layer(H, I, E, k, shared, n):
     L = _layer(H, I, E, k, shared=shared)

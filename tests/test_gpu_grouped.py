@@ -182,6 +182,32 @@ def test_streams_graphs_and_repeats(counts):
         check(y, *linear_ref(xs, w, offs, rows))
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_a_row_has_the_same_bits_in_any_batch(dtype):
+    # Decode, verify and prefill of a token agree bit for bit: K in ascending pieces of 32, whatever
+    # the tile, the batch or the alignment.
+    K, N, E = 520, 200, 3
+    x, w = randn((700, K), dtype, 101), randn((E, N, K), dtype, 102, 0.1)
+    u = randn((E, N, K), dtype, 103, 0.1)
+    off = offsets([50, 640, 10])
+    y, h = torch.empty(700, N, dtype=F32, device="cuda"), torch.empty(700, N, dtype=F32, device="cuda")
+    G.grouped_linear(x, w, off, y)
+    G.grouped_gate_up(x, w, u, off, h)
+    wide = torch.zeros(700, K + 1, dtype=dtype, device="cuda")
+    wide[:, 1:] = x
+    odd = torch.empty_like(y)
+    G.grouped_linear(wide[:, 1:], w, off, odd)
+    assert torch.equal(odd, y)
+    for r, e in ((0, 0), (49, 0), (50, 1), (333, 1), (689, 1), (690, 2), (699, 2)):
+        one = torch.empty(1, N, dtype=F32, device="cuda")
+        at = torch.tensor([r], dtype=torch.int32, device="cuda")
+        alone = offsets([1 if k == e else 0 for k in range(E)])
+        G.grouped_linear(x, w, alone, one, at)
+        assert torch.equal(one[0], y[r])
+        G.grouped_gate_up(x, w, u, alone, one, at)
+        assert torch.equal(one[0], h[r])
+
+
 def test_no_rows():
     w = randn((2, 16, 32), BF, 90)
     y = torch.empty(0, 16, dtype=BF, device="cuda")

@@ -146,16 +146,45 @@ def test_streams_graphs_and_repeats():
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
     ws = torch.empty(G.lora_workspace_bytes(n, L, K, r), dtype=torch.uint8, device="cuda")
-    xs, idv, y = x.clone(), ids.clone(), torch.empty_like(base)
+    xs, idv, y, y2 = x.clone(), ids.clone(), torch.empty_like(base), torch.empty_like(base)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         G.lora_add(xs, idv, A, B, s, base, y, ws=ws)
+        G.lora_add(xs, idv, A, B, s, base, y2)       # its workspace from the graph's pool
     for k in range(3):
         xs.copy_(randn((n, K), F32, 70 + k))
         idv.copy_(torch.randint(-1, L, (n,), generator=gen(80 + k), device="cuda").int())
         graph.replay()
         torch.cuda.synchronize()
         _check(xs, idv, A, B, s, base, None, y)
+        assert torch.equal(y, y2)
+
+
+def test_x_may_be_the_output():
+    n, L, r, K = 70, 3, 16, 264
+    x, ids, A, B, s, base, _ = _case(n, L, r, K, K, (F32, BF, F32))
+    want, z = torch.empty_like(x), x.clone()
+    G.lora_add(x, ids, A, B, s, x, want)
+    G.lora_add(z, ids, A, B, s, z, z)
+    assert torch.equal(z, want)
+    _check(x, ids, A, B, s, x, None, want)
+
+
+@pytest.mark.parametrize("n", [3, 1200])
+def test_adapters_beyond_32_bit_offsets(n):
+    # More than 2^31 elements of A before the last adapter's.
+    L, r, K, N = 8200, 128, 2048, 16
+    A = torch.empty(L, r, K, dtype=BF, device="cuda")
+    B = torch.empty(L, N, r, dtype=BF, device="cuda")
+    last = L - 1
+    A[last], B[last] = randn((r, K), BF, 1, K ** -0.5), randn((N, r), BF, 2, 0.3)
+    x, base = randn((n, K), F32, 3), randn((n, N), F32, 4)
+    ids = torch.full((n,), last, dtype=torch.int32, device="cuda")
+    ids[n // 2] = L                                   # one past the last: none
+    y = torch.empty_like(base)
+    G.lora_add(x, ids, A, B, None, base, y)
+    here = torch.where(ids == last, 0, -1).int()
+    _check(x, here, A[last:], B[last:], None, base, None, y)
 
 
 def test_python_refusals():
