@@ -88,10 +88,8 @@ template <class W>
 struct XHalf {          // x of the adapters' type
     typedef uint16_t row_t;
     typedef u32x4 frag;
-    template <bool AL>
-    static __device__ __forceinline__ frag load(const row_t* p, int k) { return load8<AL>(p, k); }
-    template <bool AL>
-    static __device__ __forceinline__ frag tail(const row_t* p, int k, int K) { return load8_tail<AL>(p, k, K); }
+    static __device__ __forceinline__ frag load(const row_t* p, int k) { return load8<false>(p, k); }
+    static __device__ __forceinline__ frag tail(const row_t* p, int k, int K) { return load8_tail<false>(p, k, K); }
     // Values 8 c .. 8 c + 7 of a step's row r at p.
     static __device__ __forceinline__ void lds(const char* p, int c, int r, frag& x) {
         x = *reinterpret_cast<const u32x4*>(p + (c ^ r) * 16);
@@ -105,21 +103,15 @@ struct XFloat {         // x fp32
     struct frag {
         float v[8];
     };
-    template <bool AL>
-    static __device__ __forceinline__ frag load(const row_t* p, int k) {
+    static __device__ __forceinline__ frag of(f32x4 a, f32x4 b) {
         frag f;
-        if constexpr (AL) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(p + k), b = *reinterpret_cast<const f32x4*>(p + k + 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { f.v[i] = a[i]; f.v[4 + i] = b[i]; }
-        } else {
-            const f32x4 a = *reinterpret_cast<const f32x4_any*>(p + k), b = *reinterpret_cast<const f32x4_any*>(p + k + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { f.v[i] = a[i]; f.v[4 + i] = b[i]; }
-        }
+        for (int i = 0; i < 4; ++i) { f.v[i] = a[i]; f.v[4 + i] = b[i]; }
         return f;
     }
-    template <bool AL>
+    static __device__ __forceinline__ frag load(const row_t* p, int k) {
+        return of(*reinterpret_cast<const f32x4_any*>(p + k), *reinterpret_cast<const f32x4_any*>(p + k + 4));
+    }
     static __device__ __forceinline__ frag tail(const row_t* p, int k, int K) {
         frag f;
 #pragma unroll
@@ -127,12 +119,8 @@ struct XFloat {         // x fp32
         return f;
     }
     static __device__ __forceinline__ void lds(const char* p, int c, int r, frag& x) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(p + ((2 * c + h) ^ r) * 16);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x.v[4 * h + i] = v[i];
-        }
+        x = of(*reinterpret_cast<const f32x4*>(p + ((2 * c) ^ r) * 16),
+               *reinterpret_cast<const f32x4*>(p + ((2 * c + 1) ^ r) * 16));
     }
     static __device__ __forceinline__ Terms3 split(const frag& x) { return split3(x.v); }
     static __device__ __forceinline__ f32x4 mma(u32x4 w, const Terms3& x, f32x4 c) { return mma3<W>(w, x, c); }
@@ -200,11 +188,11 @@ __device__ __forceinline__ int rank_of(const LoraArgs& a, int ad) {
     return a.ranks ? min(max(a.ranks[ad], 0), a.r) : a.r;
 }
 
-// part[split][t][:] = A[ids[t]][:, K of the split] x[t][K of the split]. A workgroup: 16 TB
-// tokens, 16 RB ranks, one split. A is the MFMA's A operand (D row = rank), x its B (D column = token).
+// part[split][t][:] = A[ids[t]][:, K of the split] x[t][K of the split]. A workgroup: 16 tokens,
+// 16 RB ranks, one split. A is the MFMA's A operand (D row = rank), x its B (D column = token).
 struct DownItem {
     int split, rank0, j, jn, t0, kb, ke;
-    template <int RB, int TB>
+    template <int RB>
     static __device__ __forceinline__ DownItem of(const LoraArgs& a) {
         DownItem d;
         int id = blockIdx.x;
@@ -213,7 +201,7 @@ struct DownItem {
         const int rg = a.rp / 16 > RB ? (a.rp / 16 + RB - 1) / RB : 1;
         d.rank0 = id % rg * RB * 16;
         id /= rg;
-        const BlockItem<TB> b(a, id);
+        const BlockItem<1> b(a, id);
         d.t0 = b.t0, d.j = b.j, d.jn = b.jn;
         d.kb = d.split * a.kstep;
         d.ke = min(a.K, d.kb + a.kstep);
@@ -222,136 +210,126 @@ struct DownItem {
 };
 
 // Adds the waves' sums in order and stores those of the tokens in m, ranks from rk on as zeros.
-template <int RB, int TB>
-__device__ __forceinline__ void down_store(const LoraArgs& a, const DownItem& d, const f32x4 (&acc)[RB][TB],
-                                           f32x4 (*red)[RB * TB][64], int rk, uint64_t m) {
+template <int RB>
+__device__ __forceinline__ void down_store(const LoraArgs& a, const DownItem& d, const f32x4 (&acc)[RB],
+                                           f32x4 (*red)[RB][64], int rk, uint64_t m) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
     __syncthreads();       // what red held before has been read
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-        for (int t = 0; t < TB; ++t) red[wv][b * TB + t][lane] = acc[b][t];
+    for (int b = 0; b < RB; ++b) red[wv][b][lane] = acc[b];
     __syncthreads();
-    for (int f = wv; f < RB * TB; f += kLoraWaves) {
-        const int b = f / TB, t = f % TB, row = d.rank0 + 16 * b + 4 * q, tok = d.t0 + 16 * t + r;
-        f32x4 v = red[0][f][lane];
+    for (int b = wv; b < RB; b += kLoraWaves) {
+        const int row = d.rank0 + 16 * b + 4 * q;
+        f32x4 v = red[0][b][lane];
 #pragma unroll
-        for (int w = 1; w < kLoraWaves; ++w) v += red[w][f][lane];
+        for (int w = 1; w < kLoraWaves; ++w) v += red[w][b][lane];
 #pragma unroll
         for (int c = 0; c < 4; ++c) v[c] = row + c < rk ? v[c] : 0.0f;
-        if (row < a.rp && (m >> (16 * t + r) & 1))
-            *reinterpret_cast<f32x4*>(a.part + ((long)d.split * a.n + tok) * a.rp + row) = v;
+        if (row < a.rp && (m >> r & 1))
+            *reinterpret_cast<f32x4*>(a.part + ((long)d.split * a.n + d.t0 + r) * a.rp + row) = v;
     }
 }
 
-// Rows at any address: the waves take chunks of 64 of K in turn, straight to registers.
-template <class W, class X, int RB, int TB>
+// Rows at any address: the waves take chunks of 64 of K in turn, straight to registers, the next chunk's
+// loads before this one's products.
+template <class W, class X, int RB>
 __global__ __launch_bounds__(64 * kLoraWaves, 2) void lora_down_kernel(LoraArgs a) {
     constexpr int KS = 2, KC = 32 * KS;
-    constexpr bool AL = false;
-    __shared__ f32x4 red[kLoraWaves][RB * TB][64];
+    __shared__ f32x4 red[kLoraWaves][RB][64];
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const DownItem d = DownItem::of<RB, TB>(a);
-    const int rank0 = d.rank0, t0 = d.t0, j = d.j, kb = d.kb, ke = d.ke;
-    const typename X::row_t* xp[TB];
-#pragma unroll
-    for (int t = 0; t < TB; ++t) {
-        const int tok = t0 + 16 * t + r;
-        xp[t] = static_cast<const typename X::row_t*>(a.x) + (long)(tok < a.n ? tok : t0) * a.ldx;
-    }
-    Adapters list(block_id(a, t0, 16 * TB), j);
+    const DownItem d = DownItem::of<RB>(a);
+    const typename X::row_t* xp =
+        static_cast<const typename X::row_t*>(a.x) + (long)(d.t0 + r < a.n ? d.t0 + r : d.t0) * a.ldx;
+    Adapters list(block_id(a, d.t0, 16), d.j);
     int ad;
     uint64_t m;
     while (list.next(d.jn, ad, m)) {
         const int rk = rank_of(a, ad);
-        f32x4 acc[RB][TB];
+        f32x4 acc[RB];
         const uint16_t* wp[RB];
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
             // Rows past the adapter's ranks repeat its last one and are dropped.
-            wp[b] = a.A + ((long)ad * a.r + max(min(rank0 + 16 * b + r, rk - 1), 0)) * a.K;
-#pragma unroll
-            for (int t = 0; t < TB; ++t) acc[b][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            wp[b] = a.A + ((long)ad * a.r + max(min(d.rank0 + 16 * b + r, rk - 1), 0)) * a.K;
+            acc[b] = (f32x4){0.f, 0.f, 0.f, 0.f};
         }
-        if (rk > rank0) {
+        if (rk > d.rank0) {
             struct Chunk {
                 u32x4 w[RB][KS];
-                typename X::frag x[TB][KS];
+                typename X::frag x[KS];
             };
-            auto load = [&](Chunk& c, int k) {
+            auto load = [&](Chunk& c, int k) __attribute__((always_inline)) {
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
+                    c.x[s] = X::load(xp, k + 32 * s + 8 * q);
 #pragma unroll
-                    for (int t = 0; t < TB; ++t) c.x[t][s] = X::template load<AL>(xp[t], k + 32 * s + 8 * q);
-#pragma unroll
-                    for (int b = 0; b < RB; ++b) c.w[b][s] = load8<AL>(wp[b], k + 32 * s + 8 * q);
+                    for (int b = 0; b < RB; ++b) c.w[b][s] = load8<false>(wp[b], k + 32 * s + 8 * q);
                 }
             };
-            auto mul = [&](const Chunk& c) {
+            auto mul = [&](const Chunk& c) __attribute__((always_inline)) {
 #pragma unroll
-                for (int s = 0; s < KS; ++s)
+                for (int s = 0; s < KS; ++s) {
+                    const auto x = X::split(c.x[s]);
 #pragma unroll
-                    for (int t = 0; t < TB; ++t) {
-                        const auto x = X::split(c.x[t][s]);
-#pragma unroll
-                        for (int b = 0; b < RB; ++b) acc[b][t] = X::mma(c.w[b][s], x, acc[b][t]);
-                    }
+                    for (int b = 0; b < RB; ++b) acc[b] = X::mma(c.w[b][s], x, acc[b]);
+                }
             };
             constexpr int STEP = KC * kLoraWaves;
-            int k = kb + wv * KC;
-            if (k + KC <= ke) {
+            int k = d.kb + wv * KC;
+            if (k + KC <= d.ke) {
                 Chunk c0, c1;
                 load(c0, k);
                 for (;;) {
                     k += STEP;
-                    const bool more = k + KC <= ke;
+                    const bool more = k + KC <= d.ke;
                     if (more) load(c1, k);
                     mul(c0);
                     if (!more) break;
                     k += STEP;
-                    const bool more2 = k + KC <= ke;
+                    const bool more2 = k + KC <= d.ke;
                     if (more2) load(c0, k);
                     mul(c1);
                     if (!more2) break;
                 }
             }
-            if (k < ke) {
+            if (k < d.ke) {
                 Chunk c;
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
                     const int kk = k + 32 * s + 8 * q;
+                    c.x[s] = X::tail(xp, kk, d.ke);
 #pragma unroll
-                    for (int t = 0; t < TB; ++t) c.x[t][s] = X::template tail<AL>(xp[t], kk, ke);
-#pragma unroll
-                    for (int b = 0; b < RB; ++b) c.w[b][s] = load8_tail<AL>(wp[b], kk, ke);
+                    for (int b = 0; b < RB; ++b) c.w[b][s] = load8_tail<false>(wp[b], kk, d.ke);
                 }
                 mul(c);
             }
         }
-        down_store<RB, TB>(a, d, acc, red, rk, m);
+        down_store<RB>(a, d, acc, red, rk, m);
     }
 }
 
 // The same for 16-byte aligned rows: steps of 128 of K come to LDS, x and A rows whole (256 or 512 B
 // each), D steps in a ring; wave w has K 32 w .. 32 w + 31 of each step. Chunk c (16 B) of a
-// row is at slot c ^ (row % 16): the 16 rows of a fragment fall on 16 different groups of banks.
-template <class W, class X, int RB, int TB>
-__global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 2 : 1) void lora_down_ring_kernel(LoraArgs a) {
-    constexpr int XB = sizeof(typename X::row_t), XR = 16 * TB, AR = 16 * RB;
-    constexpr int XROW = 128 * XB, XN = XR * XROW / 1024, AN = AR * 256 / 1024;     // instructions of a step
+// row is at slot c ^ (row % 16): the 16 rows of a fragment fall on 16 different groups of banks. Two
+// workgroups to a CU: with 32 tokens and one workgroup of twice the LDS, 4096 tokens of one adapter of rank
+// 64, fp32 6144 -> 2048, took 56 us instead of 47.
+template <class W, class X, int RB>
+__global__ __launch_bounds__(64 * kLoraWaves, 2) void lora_down_ring_kernel(LoraArgs a) {
+    constexpr int XB = sizeof(typename X::row_t), XROW = 128 * XB;
+    constexpr int XN = 16 * XROW / 1024, AN = 16 * RB * 256 / 1024;          // instructions of a step
     constexpr int CX = XN / kLoraWaves, CA = AN / kLoraWaves, C = CX + CA, STEP = (XN + AN) * 1024;
-    constexpr int LDS = (TB == 1 ? 80 : 160) * 1024, D0 = LDS / STEP, D = D0 < 8 ? D0 : 8;
+    constexpr int D0 = 80 * 1024 / STEP, D = D0 < 8 ? D0 : 8;
     static_assert(CX * kLoraWaves == XN && CA * kLoraWaves == AN && D >= 3, "whole instructions");
-    static_assert(kLoraWaves * RB * TB * 1024 <= D * STEP, "the sums take the ring's place");
+    static_assert(kLoraWaves * RB * 1024 <= D * STEP, "the sums take the ring's place");
     __shared__ __align__(16) char lds[D * STEP];
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const DownItem d = DownItem::of<RB, TB>(a);
+    const DownItem d = DownItem::of<RB>(a);
     const int steps = (d.ke - d.kb + 127) / 128;
     const uint32_t la = lds_addr(lds);
 
-    // This lane's part of a copy: row lane / (chunks of a row) of a piece of 1 KiB, one chunk.
+    // This lane's part of a copy: one chunk of row lane / (chunks of a row) of a piece of 1 KiB.
     constexpr int XL = XROW / 16, AL = 16;
     const char* px[CX];
     int kx[CX];                                    // the chunk's first K
@@ -362,16 +340,14 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 2 : 1) void lora_down_ri
         kx[i] = d.kb + c * 16 / XB;
         px[i] = static_cast<const char*>(a.x) + ((long)(tok < a.n ? tok : d.t0) * a.ldx + kx[i]) * XB;
     }
-    Adapters list(block_id(a, d.t0, XR), d.j);
+    Adapters list(block_id(a, d.t0, 16), d.j);
     int ad;
     uint64_t m;
     while (list.next(d.jn, ad, m)) {
         const int rk = rank_of(a, ad);
-        f32x4 acc[RB][TB];
+        f32x4 acc[RB];
 #pragma unroll
-        for (int b = 0; b < RB; ++b)
-#pragma unroll
-            for (int t = 0; t < TB; ++t) acc[b][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int b = 0; b < RB; ++b) acc[b] = (f32x4){0.f, 0.f, 0.f, 0.f};
         if (rk > d.rank0) {
             const uint16_t* pa[CA];
             int ka[CA];
@@ -382,6 +358,7 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 2 : 1) void lora_down_ri
                 ka[i] = d.kb + ((lane % AL) ^ (row % 16)) * 8;
                 pa[i] = a.A + ((long)ad * a.r + min(d.rank0 + row, rk - 1)) * a.K + ka[i];
             }
+            // Chunks past the split's K are zeros (K % 8 == 0: a chunk is inside or not).
             auto fetch = [&](int s, uint32_t slot) __attribute__((always_inline)) {
                 const int k = s * 128;
 #pragma unroll
@@ -405,10 +382,8 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 2 : 1) void lora_down_ri
                 else
                     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n s_barrier" ::: "memory");
                 u32x4 w[RB];
-                typename X::frag x[TB];
-                const char* xs = lds + cur + r * XROW;
-#pragma unroll
-                for (int t = 0; t < TB; ++t) X::lds(xs + t * 16 * XROW, 4 * wv + q, r, x[t]);
+                typename X::frag x;
+                X::lds(lds + cur + r * XROW, 4 * wv + q, r, x);
 #pragma unroll
                 for (int b = 0; b < RB; ++b)
                     w[b] = *reinterpret_cast<const u32x4*>(lds + cur + XN * 1024 + (16 * b + r) * 256 +
@@ -416,15 +391,12 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 2 : 1) void lora_down_ri
                 if (s + D - 1 < steps) fetch(s + D - 1, fill);
                 fill = cur;
                 cur = cur + STEP == D * STEP ? 0 : cur + STEP;
+                const auto xx = X::split(x);
 #pragma unroll
-                for (int t = 0; t < TB; ++t) {
-                    const auto xx = X::split(x[t]);
-#pragma unroll
-                    for (int b = 0; b < RB; ++b) acc[b][t] = X::mma(w[b], xx, acc[b][t]);
-                }
+                for (int b = 0; b < RB; ++b) acc[b] = X::mma(w[b], xx, acc[b]);
             }
         }
-        down_store<RB, TB>(a, d, acc, reinterpret_cast<f32x4 (*)[RB * TB][64]>(lds), rk, m);
+        down_store<RB>(a, d, acc, reinterpret_cast<f32x4 (*)[RB][64]>(lds), rk, m);
     }
 }
 
@@ -633,24 +605,25 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 4 : 2) void lora_up_kern
     }
 }
 
-// How the first launch splits K: into 512 workgroups (256 and 1024 of them: 4096 tokens as above 75 and 110 us
-// against 71, 64 decoding tokens of 32 adapters 22.5 and 26.7 against 23.5), 512 of K at least.
+// How the first launch splits K: into 512 workgroups (1024: 4096 tokens of 8 adapters of rank 64, fp32
+// 6144 -> 2048, 62 us against 64, but one adapter 51 against 47 and 64 decoding tokens of 32 adapters 26.7
+// against 23.5; 256: 75 for the first), 512 of K at least.
 struct LoraPlan {
-    int tb, jm, je, splits, kstep, rp;
+    int jm, je, splits, kstep, rp;
 };
 static LoraPlan plan_of(int n, int L, int K, int r) {
     LoraPlan p;
-    p.tb = n > 1024 ? 2 : 1;
     const int most = n < L ? n : L;
     // A workgroup that finds no adapter costs its start: up to 256 tokens may all be decoding, beyond
-    // most are prompts' (4096 tokens of 8 prompts and 32 decoding tokens at the end, rank 64, fp32 6144 ->
-    // 2048: 146 us with one workgroup for every block, 85 with two, 72 with two and 16 at the ends; 700 tokens
-    // of 3 prompts and 32: 22 with 16 for every block, 18 so).
-    const int jm = n <= 256 ? 16 : n <= 1024 ? 4 : 2;
+    // most are prompts' (2048 tokens of 4 prompts, rank 16, bf16 6144 -> 6144: 35 us with two workgroups for
+    // every block, 33 with one; 700 tokens of 3 prompts and 32 decoding: 22 with 16 for every block, 18
+    // with four).
+    const int jm = n <= 256 ? 16 : n <= 1024 ? 4 : 1;
     p.je = most < 16 ? most : 16;
     p.jm = p.je < jm ? p.je : jm;
     p.rp = (r + 15) / 16 * 16;
-    const long wgs = (long)((n + 16 * p.tb - 1) / (16 * p.tb)) * (n <= 256 ? p.jm : 1) * ((r + 16 * kRankBlocks - 1) / (16 * kRankBlocks));
+    const long wgs = (long)BlockItem<1>::blocks(n) * (n <= 256 ? p.jm : 1) *
+                     ((r + 16 * kRankBlocks - 1) / (16 * kRankBlocks));
     long s = (512 + wgs - 1) / wgs;
     const int top = (K + 511) / 512;
     s = s < 1 ? 1 : s > top ? top : s;
@@ -667,18 +640,14 @@ template <class W, class X>
 static void run_down(const LoraArgs& a, const LoraPlan& p, bool aligned, unsigned grid, hipStream_t s) {
     const dim3 g(grid), b(64 * kLoraWaves);
     const int rb = p.rp / 16;
-    auto go = [&](auto tb, auto r) {
-        constexpr int TB = decltype(tb)::value, RB = decltype(r)::value;
-        if (aligned) hipLaunchKernelGGL((lora_down_ring_kernel<W, X, RB, TB>), g, b, 0, s, a);
-        else hipLaunchKernelGGL((lora_down_kernel<W, X, RB, TB>), g, b, 0, s, a);
+    auto go = [&](auto r) {
+        constexpr int RB = decltype(r)::value;
+        if (aligned) hipLaunchKernelGGL((lora_down_ring_kernel<W, X, RB>), g, b, 0, s, a);
+        else hipLaunchKernelGGL((lora_down_kernel<W, X, RB>), g, b, 0, s, a);
     };
-    auto ranks = [&](auto tb) {
-        if (rb == 1) go(tb, std::integral_constant<int, 1>{});
-        else if (rb == 2) go(tb, std::integral_constant<int, 2>{});
-        else go(tb, std::integral_constant<int, 4>{});
-    };
-    if (p.tb == 1) ranks(std::integral_constant<int, 1>{});
-    else ranks(std::integral_constant<int, 2>{});
+    if (rb == 1) go(std::integral_constant<int, 1>{});
+    else if (rb == 2) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 4>{});
 }
 
 template <class W, int YD>
@@ -701,8 +670,7 @@ int launch_lora(const LoraArgs& a0, int xdt, int wdt, int ydt, hipStream_t s) {
     a.splits = p.splits, a.kstep = p.kstep, a.rp = p.rp, a.jm = p.jm, a.je = p.je;
     auto al = [](const void* q, size_t v) { return reinterpret_cast<uintptr_t>(q) % v == 0; };
     const bool aligned = a.K % 8 == 0 && al(a.x, 16) && al(a.A, 16) && a.ldx % (xdt == kF32 ? 4 : 8) == 0;
-    const long grid = (p.tb == 1 ? BlockItem<1>::count(a) : BlockItem<2>::count(a)) *
-                      ((p.rp / 16 + kRankBlocks - 1) / kRankBlocks) * p.splits;
+    const long grid = BlockItem<1>::count(a) * ((p.rp / 16 + kRankBlocks - 1) / kRankBlocks) * p.splits;
     if (grid * 64 * kLoraWaves >= (1L << 32)) return -2;   // threads of a launch
     auto down = [&](auto w) {
         using W = decltype(w);

@@ -351,7 +351,7 @@ int glmmoe_grouped_gate_up(int dtype, const void* x, int64_t ldx, int64_t x_rows
  * A x stays in fp32 and enters the second product as three bf16 terms, which hold it
  * exactly; fp32 rows of x enter the first so, too (values below 2^-110 lose their last
  * bits). One rounding, to y's type. Sums run in a fixed order.
- * Tokens of a request are expected to be neighbours: 16 to 64 consecutive tokens share
+ * Tokens of a request are expected to be neighbours: 16 or 32 consecutive tokens share
  * the weights of each adapter that occurs among them.
  * Workspace: glmmoe_lora_workspace_bytes (A x; 0 for arguments out of range), 16-byte
  * aligned; calls that may overlap need one each. n == 0 returns GLMMOE_OK. Limits:
