@@ -232,21 +232,26 @@ struct TileRun {
             }
         };
 
-        u32x4 held[AL ? 1 : CA + CB];
+        // Rows at any address: a step on its way in registers, cut at K when it goes to LDS.
+        constexpr int CH = AL ? 1 : CA + CB;
+        u32x4 held[CH];
         auto grab = [&](int s) __attribute__((always_inline)) {
-            const int k = s * kTileK;
+            const int k = s * kTileK, top = K - 8;
 #pragma unroll
-            for (int i = 0; i < CB; ++i) held[AL ? 0 : i] = load8_tail<false>(pb[i] - kb[i], k + kb[i], K);
-#pragma unroll
-            for (int i = 0; i < CA; ++i) held[AL ? 0 : CB + i] = load8_tail<false>(pa[i] - ka[i], k + ka[i], K);
+            for (int i = 0; i < CH; ++i)
+                held[i] = i < CB ? load8(pb[i] - kb[i], min(k + kb[i], top))
+                                 : load8(pa[i - CB] - ka[i - CB], min(k + ka[i - CB], top));
         };
-        auto drop = [&](uint32_t stage) __attribute__((always_inline)) {
+        auto drop = [&](int s, uint32_t stage) __attribute__((always_inline)) {
+            const int k = s * kTileK;
             char* p = lds + stage + lane * 16;
+            if (k + kTileK > K) {
 #pragma unroll
-            for (int i = 0; i < CB; ++i)
-                *reinterpret_cast<u32x4*>(p + BOFF + (W * i + wv) * 1024) = held[AL ? 0 : i];
+                for (int i = 0; i < CH; ++i) held[i] = fit8(held[i], k + (i < CB ? kb[i] : ka[i - CB]), K);
+            }
 #pragma unroll
-            for (int i = 0; i < CA; ++i) *reinterpret_cast<u32x4*>(p + at[i] * 1024) = held[AL ? 0 : CB + i];
+            for (int i = 0; i < CH; ++i)
+                *reinterpret_cast<u32x4*>(p + (i < CB ? BOFF + (W * i + wv) * 1024 : at[i - CB] * 1024)) = held[i];
         };
 
         f32x4 acc[MB][NB];
@@ -276,8 +281,14 @@ struct TileRun {
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             asm volatile("s_barrier" ::: "memory");
         } else {
-            grab(0);
-            drop(0);
+            if (K >= 8) {
+                grab(0);
+            } else {            // one step, of rows too short for a load of eight
+#pragma unroll
+                for (int i = 0; i < CH; ++i)
+                    held[i] = i < CB ? ask8(pb[i] - kb[i], 0, K) : ask8(pa[i - CB] - ka[i - CB], 0, K);
+            }
+            drop(0, 0);
             __syncthreads();
         }
         read(0, 0);
@@ -296,7 +307,7 @@ struct TileRun {
                     // Step s + 1 has arrived, and this wave's reads of step s. What may be on its way then:
                     // D - 2 steps; before step D - 2, whose x was asked for after all the first W, less.
                     if constexpr (!AL) {
-                        drop(cur ^ STAGE);      // all have read step s - 1, which was there
+                        drop(s + 1, cur ^ STAGE);   // all have read step s - 1, which was there
                         __syncthreads();
                     } else if (s + D - 1 >= steps) {
                         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n s_barrier" ::: "memory");
@@ -368,10 +379,10 @@ __global__ __launch_bounds__(512, 2) void grp_tile_kernel(GroupedArgs a) {
 }
 
 // Up to 64 rows x 128 rows of W, two workgroups of 4 waves to a CU.
-template <class T, bool DUAL, bool F32>
+template <class T, bool DUAL, bool F32, bool NT>
 __global__ __launch_bounds__(256, 2) void grp_slim_kernel(GroupedArgs a) {
     __shared__ __align__(16) char lds[80 * 1024];
-    TileRun<T, DUAL, F32, 1, 4, 2, 80 * 1024, true> t{a, lds, 0, 0, 0, 0, (int)(threadIdx.x & 63),
+    TileRun<T, DUAL, F32, 1, 4, 2, 80 * 1024, NT> t{a, lds, 0, 0, 0, 0, (int)(threadIdx.x & 63),
                                                 __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)};
     if (!find_item(a, 6, t.e, t.r0, t.nr, t.col)) return;
     if (t.nr <= 16) t.template run<1>();
@@ -379,7 +390,10 @@ __global__ __launch_bounds__(256, 2) void grp_slim_kernel(GroupedArgs a) {
     else t.template run<4>();
 }
 
-// Rows at any address: up to 64 rows x 128 rows of W, three workgroups of 4 waves to a CU.
+// Rows at any address: up to 64 rows x 128 rows of W, three workgroups of 4 waves to a CU. What bounds it: 16-byte
+// loads from odd multiples of 2 take 60 cycles of a CU's address unit for a wave, from multiples of 4 16
+// (16384 rows of 16 experts, 2047 -> 2049: 337 us, 407 TFLOP/s); more steps on their way, and aligned
+// loads whose two missing bytes come from the next lane, were no faster.
 template <class T, bool DUAL, bool F32>
 __global__ __launch_bounds__(256, 3) void grp_any_kernel(GroupedArgs a) {
     __shared__ __align__(16) char lds[48 * 1024];
@@ -402,21 +416,33 @@ static long mean_rows(const GroupedArgs& a) {
     return (rows + g - 1) / g;
 }
 
+// Large tiles up to which the slim kernel runs, too: one workgroup of it has a CU to itself, and with less
+// than two thirds of the CUs busy two smaller ones to each are faster (1332 rows of 13 experts, 1024 -> 515, 33
+// tiles: 12 us against 35; 4096 rows of 8, 4096 -> 1792, 140: 86 against 107; 4096 rows of 64, 2048 ->
+// 768, 192: 54 against 50).
+constexpr int kFewTiles = 160;
+
 template <class T, bool DUAL, bool F32>
 static int run_tiles(const GroupedArgs& a0, bool aligned, hipStream_t s) {
     GroupedArgs a = a0;
-    const bool slim = mean_rows(a) <= kSlimRows, large = aligned && !slim;
-    const int w = (large ? 256 : 128) / (DUAL ? 2 : 1);
+    const long mean = mean_rows(a), rows = (long)a.rows + a.sh_rows, groups = a.E + (a.sh_rows > 0);
+    const int wide = 256 / (DUAL ? 2 : 1);
+    // An expert's last tile is half full on average, and it has one.
+    const long g = groups < rows ? groups : rows, tiles = rows / 256 + g / 2;
+    const bool few = mean <= kSlimRows,
+               large = aligned && !few && (tiles > g ? tiles : g) * ((a.N + wide - 1) / wide) > kFewTiles;
+    const int w = large ? wide : wide / 2;
     a.ntn = (a.N + w - 1) / w;
     // More rows: the tiles of an expert share its W. Fewer: W is read once and keeps out of L2.
-    a.fours = mean_rows(a) > 256;
+    a.fours = mean > 256;
     const long items = grid_items(a, large ? 256 : 64);
     if (items * 512 >= (1L << 32)) return -2;     // threads of a launch
     const dim3 grid((unsigned)items);
     if (large && a.fours) hipLaunchKernelGGL((grp_tile_kernel<T, DUAL, F32, false>), grid, dim3(512), 0, s, a);
     else if (large) hipLaunchKernelGGL((grp_tile_kernel<T, DUAL, F32, true>), grid, dim3(512), 0, s, a);
-    else if (aligned) hipLaunchKernelGGL((grp_slim_kernel<T, DUAL, F32>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((grp_any_kernel<T, DUAL, F32>), grid, dim3(256), 0, s, a);
+    else if (!aligned) hipLaunchKernelGGL((grp_any_kernel<T, DUAL, F32>), grid, dim3(256), 0, s, a);
+    else if (few) hipLaunchKernelGGL((grp_slim_kernel<T, DUAL, F32, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((grp_slim_kernel<T, DUAL, F32, false>), grid, dim3(256), 0, s, a);
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }
 

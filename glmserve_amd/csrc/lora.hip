@@ -88,8 +88,8 @@ template <class W>
 struct XHalf {          // x of the adapters' type
     typedef uint16_t row_t;
     typedef u32x4 frag;
-    static __device__ __forceinline__ frag load(const row_t* p, int k) { return load8<false>(p, k); }
-    static __device__ __forceinline__ frag tail(const row_t* p, int k, int K) { return load8_tail<false>(p, k, K); }
+    static __device__ __forceinline__ frag load(const row_t* p, int k) { return load8(p, k); }
+    static __device__ __forceinline__ frag tail(const row_t* p, int k, int K) { return load8_tail(p, k, K); }
     // Values 8 c .. 8 c + 7 of a step's row r at p.
     static __device__ __forceinline__ void lds(const char* p, int c, int r, frag& x) {
         x = *reinterpret_cast<const u32x4*>(p + (c ^ r) * 16);
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(64 * kLoraWaves, 2) void lora_down_kernel(LoraArgs 
                 for (int s = 0; s < KS; ++s) {
                     c.x[s] = X::load(xp, k + 32 * s + 8 * q);
 #pragma unroll
-                    for (int b = 0; b < RB; ++b) c.w[b][s] = load8<false>(wp[b], k + 32 * s + 8 * q);
+                    for (int b = 0; b < RB; ++b) c.w[b][s] = load8(wp[b], k + 32 * s + 8 * q);
                 }
             };
             auto mul = [&](const Chunk& c) __attribute__((always_inline)) {
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(64 * kLoraWaves, 2) void lora_down_kernel(LoraArgs 
                     const int kk = k + 32 * s + 8 * q;
                     c.x[s] = X::tail(xp, kk, d.ke);
 #pragma unroll
-                    for (int b = 0; b < RB; ++b) c.w[b][s] = load8_tail<false>(wp[b], kk, d.ke);
+                    for (int b = 0; b < RB; ++b) c.w[b][s] = load8_tail(wp[b], kk, d.ke);
                 }
                 mul(c);
             }
@@ -405,9 +405,6 @@ template <int DT>
 struct Out {
     typedef uint16_t elem;
     static __device__ __forceinline__ float get(const elem* p) { return DT == kBf16 ? Bf16::up(*p) : F16::up(*p); }
-    static __device__ __forceinline__ void put(elem* p, float v) {
-        *p = (uint16_t)(DT == kBf16 ? Bf16::pack2(v, v) : F16::pack2(v, v));
-    }
     static __device__ __forceinline__ f32x4 get4(const elem* p) {
         const u32x2 w = *reinterpret_cast<const u32x2_any*>(p);
         f32x4 v;
@@ -418,25 +415,23 @@ struct Out {
         }
         return v;
     }
-    static __device__ __forceinline__ void put4(elem* p, f32x4 v) {
-        if constexpr (DT == kBf16) store4<Bf16, false>(p, 0, v, 4);
-        else store4<F16, false>(p, 0, v, 4);
+    static __device__ __forceinline__ void put(elem* p, f32x4 v, int cnt) {
+        if constexpr (DT == kBf16) store4<Bf16, false>(p, 0, v, cnt);
+        else store4<F16, false>(p, 0, v, cnt);
     }
 };
 template <>
 struct Out<kF32> {
     typedef float elem;
     static __device__ __forceinline__ float get(const float* p) { return *p; }
-    static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
     static __device__ __forceinline__ f32x4 get4(const float* p) { return *reinterpret_cast<const f32x4_any*>(p); }
-    static __device__ __forceinline__ void put4(float* p, f32x4 v) { *reinterpret_cast<f32x4_any*>(p) = v; }
+    static __device__ __forceinline__ void put(float* p, f32x4 v, int cnt) { store4<Bf16, true>(p, 0, v, cnt); }
 };
 
 // y = base + scale * B (sum of part over the splits). A workgroup: 16 TB tokens, 256
 // columns, 64 per wave; A x is summed, cut into three bf16 terms and kept in LDS, while the first
 // adapter's rows of B and its tokens' base are on their way. B is the MFMA's A operand (D row =
-// output), A x its B (D column = token): a lane has four neighbouring outputs of one token. The up to
-// three columns after N's last four are plain dot products.
+// output), A x its B (D column = token): a lane has four neighbouring outputs of one token.
 template <class W, int YD, int TB>
 __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 4 : 2) void lora_up_kernel(LoraArgs a) {
     constexpr int NB = 4;
@@ -454,7 +449,7 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 4 : 2) void lora_up_kern
     const uint64_t here = left >= 64 ? ~0ull : (1ull << left) - 1;
     const int id0 = lane < left ? a.ids[t0 + lane] : -1;
 
-    const int n4 = a.N & ~3, nl = n0 + 4 * q;                    // whole fours; the lane's first column
+    const int nl = n0 + 4 * q;                                   // the lane's first column
     const elem* pb = static_cast<const elem*>(a.base) + (long)(t0 + r) * a.ldb + nl;
     elem* py = static_cast<elem*>(a.y) + (long)(t0 + r) * a.ldy + nl;
     f32x4 base[TB][NB];
@@ -466,11 +461,11 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 4 : 2) void lora_up_kern
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 w[b] = (u32x4){0u, 0u, 0u, 0u};
-                if (k + 8 * q < rk) w[b] = load8<false>(wp[b], k + 8 * q);
+                if (k + 8 * q < rk) w[b] = load8(wp[b], k + 8 * q);
             }
         } else {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) w[b] = load8_tail<false>(wp[b], k + 8 * q, rk);
+            for (int b = 0; b < NB; ++b) w[b] = load8_tail(wp[b], k + 8 * q, rk);
         }
     };
     auto load_base = [&](uint64_t mask) __attribute__((always_inline)) {
@@ -479,8 +474,16 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 4 : 2) void lora_up_kern
             if (mask >> (16 * t + r) & 1) {
                 const elem* p = pb + 16L * t * a.ldb;
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
-                    if (nl + 16 * b < n4) base[t][b] = O::get4(p + 16 * b);
+                for (int b = 0; b < NB; ++b) {
+                    const int cnt = a.N - nl - 16 * b;           // of its four columns, those inside N
+                    if (cnt >= 4) {
+                        base[t][b] = O::get4(p + 16 * b);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 3; ++c)
+                            if (c < cnt) base[t][b][c] = O::get(p + 16 * b + c);
+                    }
+                }
             }
     };
     // The workgroups that all blocks have ask for the block's base and A x before they know its adapters.
@@ -541,7 +544,6 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 4 : 2) void lora_up_kern
     }
     __syncthreads();
 
-    const bool last = n4 < a.N && n0 <= n4 && n4 < n0 + 16 * NB;   // this wave has N's last columns
     while (some) {
         const float sc = a.scale ? a.scale[ad] : 1.0f;
         f32x4 acc[NB][TB];
@@ -567,24 +569,12 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 4 : 2) void lora_up_kern
                 elem* p = py + 16L * t * a.ldy;
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
-                    if (nl + 16 * b < n4) {
+                    if (nl + 16 * b < a.N) {
                         f32x4 v;
 #pragma unroll
                         for (int c = 0; c < 4; ++c) v[c] = __builtin_fmaf(sc, acc[b][t][c], base[t][b][c]);
-                        O::put4(p + 16 * b, v);
+                        O::put(p + 16 * b, v, a.N - nl - 16 * b);
                     }
-            }
-        if (last && lane < 16 * TB && (m >> lane & 1))
-            for (int n = n4; n < a.N; ++n) {
-                const uint16_t* row = a.B + ((long)ad * a.N + n) * a.r;
-                float v = 0.0f;
-                for (int k = 0; k < rk; ++k) {
-                    const uint16_t* t = terms + lane * stride + k;
-                    const float x = (Bf16::up(t[0]) + Bf16::up(t[16 * TB * stride])) + Bf16::up(t[32 * TB * stride]);
-                    v = __builtin_fmaf(W::up(row[k]), x, v);
-                }
-                const elem* p = static_cast<const elem*>(a.base) + (long)(t0 + lane) * a.ldb + n;
-                O::put(static_cast<elem*>(a.y) + (long)(t0 + lane) * a.ldy + n, __builtin_fmaf(sc, v, O::get(p)));
             }
         some = list.next(jn, ad, m);
         if (some) begin();
@@ -596,12 +586,8 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 4 : 2) void lora_up_kern
                 elem* p = py + 16L * t * a.ldy;
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
-                    if (nl + 16 * b < n4) O::put4(p + 16 * b, base[t][b]);
+                    if (nl + 16 * b < a.N) O::put(p + 16 * b, base[t][b], a.N - nl - 16 * b);
             }
-        if (last && lane < 16 * TB && (none >> lane & 1))
-            for (int n = n4; n < a.N; ++n)
-                static_cast<elem*>(a.y)[(long)(t0 + lane) * a.ldy + n] =
-                    static_cast<const elem*>(a.base)[(long)(t0 + lane) * a.ldb + n];
     }
 }
 

@@ -22,10 +22,6 @@ struct Bf16 {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                        __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
-                                                       __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    }
     static __device__ __forceinline__ uint32_t pack2(float a, float b) { return pack_bf16x2(a, b); }
     static __device__ __forceinline__ float up(uint32_t h) { return bf16_to_f32(h & 0xffffu); }
 };
@@ -34,10 +30,6 @@ struct F16 {
     static constexpr int code = kF16;
     static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
-                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    }
-    static __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
                                                       __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
     // Round to nearest even, as the hardware conversion does.
@@ -49,30 +41,33 @@ struct F16 {
     }
 };
 
-// 8 values k .. k + 7 of a row, all inside it. AL: 16-byte aligned.
-template <bool AL, bool NT = false>
+// 8 values k .. k + 7 of a row, all inside it.
 __device__ __forceinline__ u32x4 load8(const uint16_t* row, int k) {
-    if constexpr (AL) {
-        const u32x4* p = reinterpret_cast<const u32x4*>(row + k);
-        if constexpr (NT) return __builtin_nontemporal_load(p);
-        return *p;
-    } else {
-        return *reinterpret_cast<const u32x4_any*>(row + k);
-    }
+    return *reinterpret_cast<const u32x4_any*>(row + k);
 }
 
-// The same with zeros from K on. AL: K is a multiple of 8.
-template <bool AL>
-__device__ __forceinline__ u32x4 load8_tail(const uint16_t* row, int k, int K) {
-    if (k + 8 <= K) return load8<AL>(row, k);
+// The same of a row of K values, with zeros from K on. ask8: the eight that end at K instead, where the row ends
+// before k + 8 (a row of fewer has them one by one); fit8 makes of them what was asked for. Loads and
+// their use stay apart so, without a branch between them.
+__device__ __forceinline__ u32x4 ask8(const uint16_t* row, int k, int K) {
+    if (K >= 8) return load8(row, min(k, K - 8));
     u32x4 v = {0u, 0u, 0u, 0u};
-    if constexpr (!AL) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (k + i < K) v[i / 2] |= (uint32_t)row[k + i] << (16 * (i & 1));
-    }
+    for (int i = 0; i < 7; ++i)
+        if (i < K) v[i / 2] |= (uint32_t)row[i] << (16 * (i & 1));
     return v;
 }
+__device__ __forceinline__ u32x4 fit8(u32x4 v, int k, int K) {
+    const int over = min(max(k - max(K - 8, 0), 0), 8);      // values before k; K < 8: k is a multiple of 8
+    uint64_t lo = v[0] | (uint64_t)v[1] << 32, hi = v[2] | (uint64_t)v[3] << 32;
+    if (over & 4) lo = hi, hi = 0;
+    const int sh = (over & 3) * 16;
+    lo = sh ? lo >> sh | hi << (64 - sh) : lo;
+    hi >>= sh;
+    if (over == 8) lo = 0, hi = 0;
+    return (u32x4){(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+}
+__device__ __forceinline__ u32x4 load8_tail(const uint16_t* row, int k, int K) { return fit8(ask8(row, k, K), k, K); }
 
 // 16 bytes of zeros in memory, for copies of what lies past a row's end.
 static __device__ const u32x4 kZero16 = {0u, 0u, 0u, 0u};

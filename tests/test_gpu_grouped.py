@@ -58,6 +58,52 @@ def test_gate_up(counts, N, K, dtype, out):
     check(h, *gate_up_ref(x, wg, wu, offsets(counts), rows, ids))
 
 
+# So many columns that the large tiles fill the GPU: W read once, and shared by an expert's tiles, the last ones in
+# halves of the columns.
+WIDE = [MANY, [600, 0, 900, 257]]
+
+
+@pytest.mark.parametrize("dtype,out", [(BF, BF), (FP, F32)])
+@pytest.mark.parametrize("counts", WIDE, ids=["once", "shared"])
+@pytest.mark.parametrize("K", [72, 264])
+def test_large_tiles(counts, K, dtype, out):
+    _linear(counts, 5300, K, dtype, out, 91, gather=K == 72, first=3, after=5)
+
+
+@pytest.mark.parametrize("dtype,out", [(FP, FP), (BF, F32)])
+@pytest.mark.parametrize("counts", WIDE, ids=["once", "shared"])
+def test_large_tiles_gate_up(counts, dtype, out):
+    rows, E, K, N = sum(counts), len(counts), 136, 2700
+    x = randn((rows, K), dtype, 92)
+    wg, wu = randn((E, N, K), dtype, 93, 2 * K ** -0.5), randn((E, N, K), dtype, 94, K ** -0.5)
+    h = torch.empty(rows, N, dtype=out, device="cuda")
+    G.grouped_gate_up(x, wg, wu, offsets(counts), h)
+    check(h, *gate_up_ref(x, wg, wu, offsets(counts), rows))
+
+
+@pytest.mark.parametrize("counts", WIDE, ids=["once", "shared"])
+def test_large_tiles_bad_ids_not_finite_and_bits(counts):
+    rows, K, N = sum(counts), 128, 5300
+    x, w, off = randn((50, K), BF, 95), randn((len(counts), N, K), BF, 96, 0.1), offsets(counts)
+    ids = torch.randint(0, 49, (rows,), generator=gen(97), device="cuda").int()
+    ids[0], ids[299], ids[rows - 1], ids[5] = -1, 50, 2 ** 31 - 1, 49
+    x[49, 7] = float("nan")
+    y = torch.full((rows, N), 7.0, dtype=F32, device="cuda")
+    G.grouped_linear(x, w, off, y, ids)
+    assert torch.isnan(y[5]).all()
+    for r in (0, 299, rows - 1):
+        assert torch.all(y[r] == 0)
+    ref, err, live = linear_ref(x, w, off, rows, ids)
+    live[5] = False
+    check(y, ref, err, live)
+    again = torch.empty_like(y)
+    G.grouped_linear(x, w, off, again, ids)
+    part = torch.empty(rows, 64, dtype=F32, device="cuda")       # few columns: the small tiles
+    G.grouped_linear(x, w[:, :64].contiguous(), off, part, ids)
+    live[5] = False
+    assert torch.equal(again[live], y[live]) and torch.equal(part[live], y[live][:, :64])
+
+
 def test_many_experts():
     # More experts than lanes, most of them empty, groups far apart.
     counts = [0] * 700
