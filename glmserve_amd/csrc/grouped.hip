@@ -417,7 +417,7 @@ static long mean_rows(const GroupedArgs& a) {
 }
 
 // Large tiles up to which the slim kernel runs, too: one workgroup of it has a CU to itself, and with less
-// than two thirds of the CUs busy two smaller ones to each are faster (1332 rows of 13 experts, 1024 -> 515, 33
+// than two thirds of the CUs busy two smaller ones to each are faster (1332 rows of 13 experts, 1024 -> 515, 39
 // tiles: 12 us against 35; 4096 rows of 8, 4096 -> 1792, 140: 86 against 107; 4096 rows of 64, 2048 ->
 // 768, 192: 54 against 50).
 constexpr int kFewTiles = 160;

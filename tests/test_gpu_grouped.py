@@ -44,6 +44,11 @@ def test_linear_odd_sizes(counts, N, K):
     _linear(counts, N, K, FP, F32, N + K, gather=True)
 
 
+@pytest.mark.parametrize("K", [2, 4, 5, 6, 9, 10, 11, 12, 13, 14, 15, 66, 67, 68, 69, 70, 71, 127])
+def test_linear_every_row_end(K):
+    _linear([3, 0, 70], 37, K, BF, F32, K)
+
+
 @pytest.mark.parametrize("dtype,out", [(BF, BF), (FP, FP), (BF, F32)])
 @pytest.mark.parametrize("counts", [[1], FEW, MID, MANY], ids=["one", "few", "mid", "many"])
 @pytest.mark.parametrize("N,K", [(128, 256), (260, 1064), (67, 131)])

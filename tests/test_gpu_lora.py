@@ -60,6 +60,12 @@ def test_sizes(K, N, n):
     _run(n, 4, 10, K, N, (BF, BF, BF))
 
 
+@pytest.mark.parametrize("K", [2, 4, 5, 6, 9, 10, 11, 12, 13, 14, 15, 66, 68, 69, 70, 255])
+def test_every_row_end(K):
+    _run(21, 4, K % 9 + 1, K, K, (BF, BF, BF))
+    _run(21, 4, 16 + K % 8, 530 + K, 64 + K, (F32, FP, F32))
+
+
 @pytest.mark.parametrize("n", [64, 600, 1500])
 def test_adapter_patterns(n):
     t = (F32, BF, F32)
