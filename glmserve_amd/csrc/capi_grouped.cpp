@@ -79,7 +79,7 @@ int glmmoe_grouped_gate_up(int dtype, const void* x, int64_t ldx, int64_t x_rows
 
 size_t glmmoe_lora_workspace_bytes(int n, int n_adapters, int64_t K, int r) {
     if (n <= 0 || n_adapters <= 0 || K <= 0 || r <= 0 || !lora_shape_ok(n, n_adapters, K, r)) return 0;
-    return lora_part_bytes(n, n_adapters, (int)K, r);
+    return lora_part_bytes(n, (int)K, r);
 }
 
 int glmmoe_lora_add(int x_dtype, const void* x, int64_t ldx, const int* adapter_ids, int n,

@@ -45,7 +45,7 @@ struct LoraArgs {
     int splits, kstep, rp;    // set by the launch: K per split, row length of part,
     int jm, je, nx;           // workgroups per token block (by adapter), at both ends; along N
 };
-size_t lora_part_bytes(int n, int L, int K, int r);
+size_t lora_part_bytes(int n, int K, int r);
 int launch_lora(const LoraArgs& a, int xdt, int wdt, int ydt, hipStream_t s);
 
 }  // namespace glmmoe

@@ -594,6 +594,7 @@ __global__ __launch_bounds__(64 * kLoraWaves, TB == 1 ? 4 : 2) void lora_up_kern
 // How the first launch splits K: into 512 workgroups (1024: 4096 tokens of 8 adapters of rank 64, fp32
 // 6144 -> 2048, 62 us against 64, but one adapter 51 against 47 and 64 decoding tokens of 32 adapters 26.7
 // against 23.5; 256: 75 for the first), 512 of K at least.
+constexpr int kDownGroups = 512;
 struct LoraPlan {
     int jm, je, splits, kstep, rp;
 };
@@ -610,16 +611,19 @@ static LoraPlan plan_of(int n, int L, int K, int r) {
     p.rp = (r + 15) / 16 * 16;
     const long wgs = (long)BlockItem<1>::blocks(n) * (n <= 256 ? p.jm : 1) *
                      ((r + 16 * kRankBlocks - 1) / (16 * kRankBlocks));
-    long s = (512 + wgs - 1) / wgs;
+    long s = (kDownGroups + wgs - 1) / wgs;
     const int top = (K + 511) / 512;
     s = s < 1 ? 1 : s > top ? top : s;
     p.kstep = (int)(((K + s - 1) / s + 127) / 128 * 128);
     p.splits = (K + p.kstep - 1) / p.kstep;
     return p;
 }
-size_t lora_part_bytes(int n, int L, int K, int r) {
-    const LoraPlan p = plan_of(n, L, K, r);
-    return (size_t)p.splits * n * p.rp * 4;
+// What any plan of these sizes or smaller ones takes: splits < kDownGroups / wgs + 1 and wgs >= n / 16, so splits * n
+// < 16 kDownGroups + n; and no more than K's own limit. A plan's own need is not monotone (8176 tokens
+// have two splits, 8192 one), and a workspace for the most tokens has to serve fewer.
+size_t lora_part_bytes(int n, int K, int r) {
+    const size_t all = (size_t)n * ((K + 511) / 512), most = (size_t)16 * kDownGroups + n;
+    return (all < most ? all : most) * ((r + 15) / 16 * 16) * 4;
 }
 
 template <class W, class X>

@@ -353,8 +353,9 @@ int glmmoe_grouped_gate_up(int dtype, const void* x, int64_t ldx, int64_t x_rows
  * bits). One rounding, to y's type. Sums run in a fixed order.
  * Tokens of a request are expected to be neighbours: 16 or 32 consecutive tokens share
  * the weights of each adapter that occurs among them.
- * Workspace: glmmoe_lora_workspace_bytes (A x; 0 for arguments out of range), 16-byte
- * aligned; calls that may overlap need one each. n == 0 returns GLMMOE_OK. Limits:
+ * Workspace: glmmoe_lora_workspace_bytes (A x; 0 for arguments out of range; never less
+ * for more tokens, a longer K or a larger rank), 16-byte aligned; calls that may overlap
+ * need one each. n == 0 returns GLMMOE_OK. Limits:
  * r <= 256, n < 2^24, n_adapters <= 2^24, K and N < 2^24. */
 size_t glmmoe_lora_workspace_bytes(int n, int n_adapters, int64_t K, int r);
 int glmmoe_lora_add(int x_dtype, const void* x, int64_t ldx, const int* adapter_ids, int n,

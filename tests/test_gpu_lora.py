@@ -166,6 +166,19 @@ def test_streams_graphs_and_repeats():
         assert torch.equal(y, y2)
 
 
+def test_a_workspace_for_more_tokens():
+    # 8192 tokens take one pass over K, 8176 two: the workspace of the former serves both, to its end.
+    L, r, K, N = 3, 16, 1024, 64
+    x, ids, A, B, s, base, _ = _case(8192, L, r, K, N, (BF, BF, BF))
+    nb = G.lora_workspace_bytes(8192, L, K, r)
+    ws = torch.full((nb + 4096,), 7, dtype=torch.uint8, device="cuda")
+    for n in (8176, 8192, 4097, 300, 1):
+        y = torch.empty_like(base[:n])
+        G.lora_add(x[:n], ids[:n], A, B, s, base[:n], y, ws=ws[:nb])
+        _check(x[:n], ids[:n], A, B, s, base[:n], None, y)
+        assert torch.all(ws[nb:] == 7)
+
+
 def test_x_may_be_the_output():
     n, L, r, K = 70, 3, 16, 264
     x, ids, A, B, s, base, _ = _case(n, L, r, K, K, (F32, BF, F32))

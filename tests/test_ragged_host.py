@@ -149,3 +149,14 @@ def test_checkpoint_in_bf16(tmp_path):
     save_file(t, f)
     with pytest.raises(G.GlmMoeError):
         read_layer(f, 0, experts="bf16")
+
+
+@pytest.mark.parametrize("K,r", [(1000, 12), (6144, 64), (6144, 256)])
+def test_lora_workspace_of_more_tokens_is_enough_for_fewer(K, r):
+    f, last = _lib.lib().glmmoe_lora_workspace_bytes, 0
+    for n in range(1, 20001):
+        need = f(n, 32, K, r)
+        assert need >= last, n
+        last = need
+    for n in (1, 64, 1000, 8176):
+        assert f(n, 4, K, r) == f(n, 32, K, r) >= f(n, 32, K - 500, r) and f(n, 32, K, r) >= f(n, 32, K, r - 5)
