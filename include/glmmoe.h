@@ -406,6 +406,8 @@ typedef struct glmmoe_bf16_ws {
     size_t bytes;
 } glmmoe_bf16_ws;
 
+/* Bytes for n tokens; the routing's scratch has steps (256, 1025, 2049, 4097 tokens) where one
+ * token more takes less, so a workspace for several n takes the largest of their sizes. */
 size_t glmmoe_bf16_layer_workspace_bytes(const glmmoe_bf16_layer* L, int n);
 int glmmoe_bf16_layer_workspace_view(const glmmoe_bf16_layer* L, int n, void* workspace,
                                      glmmoe_bf16_ws* view);
